@@ -297,6 +297,134 @@ int ssa_sparse_gather_attention_bwd_det(const ssa_apply_bwd_args *a, void *works
                                         int64_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Serving from a paged 8-bit key/value cache (no counterpart in the reference,
+ * which recomputes the prefix for every token).
+ *
+ * A page holds `page` tokens (32, 64 or 128) of every kv head as OCP e4m3 codes,
+ * with one power-of-two scale per (page, head) for the keys and one for the
+ * values; a number is code * scale.  D, the stored head dim, is d rounded up to
+ * 64, 128 or 256 (zero codes in the added columns).  The value codes lie
+ * transposed, so that the attention's second product reads them as its matrix
+ * operand.  All buffers are contiguous and 16-byte aligned, and the caller's;
+ * value codes are never NaN (ssa_cache_append writes none; a new cache is
+ * zeroed).
+ *
+ * A batch is ragged: request r's pages are block_table[r][0..width), its new
+ * rows starts[r] .. starts[r+1]-1.  A page id outside [0, num_pages) is an
+ * absent page: its keys are not seen.
+ * --------------------------------------------------------------------------- */
+typedef struct {
+    void *k_codes;           /* (num_pages, Hkv, page, D) */
+    void *v_codes;           /* (num_pages, Hkv, D, page) */
+    void *bounds;            /* (num_pages, Hkv, 2, D): per channel the smallest and   */
+                             /* the largest key code appended since the page was begun */
+    float *k_scale, *v_scale;/* (num_pages, Hkv) */
+    int64_t num_pages;
+    int32_t Hkv, page, D, d;
+} ssa_kv_cache;
+
+typedef struct {
+    const int32_t *block_table;  /* (R, width) */
+    int64_t table_stride;        /* elements between its rows */
+    int32_t R, width;
+    const int32_t *starts;       /* R + 1, ascending */
+    const int32_t *requests;     /* T: request of each row, -1 for none */
+    const int32_t *positions;    /* T: index of each row's token in its request, -1 for none */
+    int32_t T;
+} ssa_batch_rows;
+
+/* Block tables, slots and positions of a batch from its requests' lengths.
+ * Request r holds cached[r] tokens and brings new_rows[r]; its rows follow those
+ * of r-1.  It is admitted when its rows lie within the T rows, its tokens fit
+ * `width` pages, its lengths are not negative, and the pages that it and all
+ * earlier such requests need are free (or it needs none).  The k-th page taken is
+ * free_pages[free_count - 1 - k].  Writes the new pages into block_table (its
+ * other entries are only read), and
+ *   starts R+1; lengths R (cached, plus new_rows where admitted); per row the
+ *   slot page * page_size + offset, the position and the request (all -1 in rows
+ *   of a refused request or of none); free_count_out 1; refused 1 (a count).
+ * R up to 16,384; one launch. */
+typedef struct {
+    const int32_t *cached, *new_rows;    /* R */
+    int32_t *block_table;                /* (R, width) */
+    int64_t table_stride;
+    int32_t R, width, page, T;
+    const int32_t *free_pages;           /* free_capacity */
+    int32_t free_capacity;
+    const int32_t *free_count;           /* 1 */
+    int32_t *starts, *lengths;
+    int64_t *slots;
+    int32_t *positions, *requests, *free_count_out, *refused;
+} ssa_page_plan_args;
+
+int ssa_page_plan(const ssa_page_plan_args *a, void *stream);
+
+/* Writes T rows of keys and values (T, Hkv, d; SSA_F32 / SSA_BF16 / SSA_F16, unit
+ * last stride, row and head strides in elements) into the cache at slots[t] =
+ * page * page_size + offset (outside the cache: the row is skipped).  A page's
+ * rows in one call are adjacent and ascend by one; its tokens below the first of
+ * them stay, those from it on are given up.  The page's scale is the larger of
+ * its own (unless the rows begin the page) and the smallest power of two with
+ * |x| <= 448 scale for all x of the rows, at least 2^-100; where it grows, the
+ * codes that stay and the bounds are rounded to it.  Codes are rounded to
+ * nearest, ties to even.  A row with a NaN, an infinity or a magnitude of 2^120
+ * or more in a head's key or value is stored as NaN key codes and zero value
+ * codes of that head (and as NaN bounds): a query that sees it is NaN, no
+ * other. */
+typedef struct {
+    ssa_kv_cache cache;
+    const void *k, *v;
+    int32_t dtype, T;
+    int64_t k_st, k_sh, v_st, v_sh;
+    const int64_t *slots;
+} ssa_cache_append_args;
+
+int ssa_cache_append(const ssa_cache_append_args *a, void *stream);
+
+/* For each row and kv head the `top_k` pages to attend to, of the row's n =
+ * position / page + 1: the first `first` and the last `recent` (>= 1) of them, and
+ * of the others those with the largest
+ *   sum over the head's query heads g and channels c of
+ *       max(q[g][c] * lo[c], q[g][c] * hi[c])          (lo, hi: the page's bounds),
+ * an upper bound of the sum of the group's scores with any one key of the page, in
+ * fp64; NaN ranks as +inf, ties go to the lower page, an absent page ranks last.
+ * out (T, Hkv, top_k) int32: pages of the request in ascending order, then -1. */
+typedef struct {
+    ssa_kv_cache cache;
+    ssa_batch_rows rows;
+    const void *q;                       /* (T, Hq, d) */
+    int32_t dtype, Hq;
+    int64_t q_st, q_sh;
+    int32_t top_k, first, recent;
+    int32_t *out;
+} ssa_select_pages_args;
+
+int ssa_select_pages(const ssa_select_pages_args *a, void *stream);
+
+/* out[t][g] = sum_j p_j v_j, p = softmax(scale * q[t][g] . k_j) over the keys j <=
+ * positions[t] of the row's request, all of them or those of `pages` (T, Hkv, top;
+ * negative: none; each page at most once).  q and out (T, Hq, d), unit last
+ * strides; out in q's type.  Query head g reads kv head g / (Hq / Hkv).  Products
+ * of q and codes are exact, sums and softmax in fp32, probabilities to 16 bits
+ * (24 for fp32 q).  A row that sees no key gets zeros.  Needs a 16-byte aligned
+ * workspace of ssa_cached_attention_workspace_bytes (0 for some sizes). */
+typedef struct {
+    ssa_kv_cache cache;
+    ssa_batch_rows rows;
+    const void *q;
+    void *out;
+    int32_t dtype, Hq;
+    int64_t q_st, q_sh, o_st, o_sh;
+    float scale;
+    const int32_t *pages;                /* NULL: all keys */
+    int32_t top;
+} ssa_cached_attention_args;
+
+int64_t ssa_cached_attention_workspace_bytes(const ssa_cached_attention_args *a);
+int ssa_cached_attention(const ssa_cached_attention_args *a, void *workspace,
+                         int64_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
  * Measurement helper (no counterpart in the reference): the L2-to-CU delivery
  * rate that bounds the gather attention, whose repeated K/V rows are served by
  * the L2 rather than HBM.  `blocks` workgroups of 256 threads each stream the

@@ -75,6 +75,45 @@ class ApplyGradArgs(ctypes.Structure):
                 ("dv", Tensor4), ("deterministic", c_i32)]
 
 
+class KVCacheStruct(ctypes.Structure):
+    _fields_ = [("k_codes", c_vp), ("v_codes", c_vp), ("bounds", c_vp),
+                ("k_scale", c_vp), ("v_scale", c_vp), ("num_pages", c_i64),
+                ("Hkv", c_i32), ("page", c_i32), ("D", c_i32), ("d", c_i32)]
+
+
+class BatchRows(ctypes.Structure):
+    _fields_ = [("block_table", c_vp), ("table_stride", c_i64), ("R", c_i32), ("width", c_i32),
+                ("starts", c_vp), ("requests", c_vp), ("positions", c_vp), ("T", c_i32)]
+
+
+class PagePlanArgs(ctypes.Structure):
+    _fields_ = [("cached", c_vp), ("new_rows", c_vp), ("block_table", c_vp),
+                ("table_stride", c_i64), ("R", c_i32), ("width", c_i32), ("page", c_i32),
+                ("T", c_i32), ("free_pages", c_vp), ("free_capacity", c_i32),
+                ("free_count", c_vp), ("starts", c_vp), ("lengths", c_vp), ("slots", c_vp),
+                ("positions", c_vp), ("requests", c_vp), ("free_count_out", c_vp),
+                ("refused", c_vp)]
+
+
+class CacheAppendArgs(ctypes.Structure):
+    _fields_ = [("cache", KVCacheStruct), ("k", c_vp), ("v", c_vp), ("dtype", c_i32),
+                ("T", c_i32), ("k_st", c_i64), ("k_sh", c_i64), ("v_st", c_i64), ("v_sh", c_i64),
+                ("slots", c_vp)]
+
+
+class SelectPagesArgs(ctypes.Structure):
+    _fields_ = [("cache", KVCacheStruct), ("rows", BatchRows), ("q", c_vp), ("dtype", c_i32),
+                ("Hq", c_i32), ("q_st", c_i64), ("q_sh", c_i64), ("top_k", c_i32),
+                ("first", c_i32), ("recent", c_i32), ("out", c_vp)]
+
+
+class CachedAttentionArgs(ctypes.Structure):
+    _fields_ = [("cache", KVCacheStruct), ("rows", BatchRows), ("q", c_vp), ("out", c_vp),
+                ("dtype", c_i32), ("Hq", c_i32), ("q_st", c_i64), ("q_sh", c_i64),
+                ("o_st", c_i64), ("o_sh", c_i64), ("scale", ctypes.c_float), ("pages", c_vp),
+                ("top", c_i32)]
+
+
 _lib = None
 _override = None
 CHECKED_LIB_PATH = os.path.join(_HERE, "libssa_amd_checked.so")
@@ -178,6 +217,16 @@ def _configure(L):
     L.ssa_sparse_gather_attention_grad.restype = ctypes.c_int
     L.ssa_sparse_gather_attention_grad.argtypes = [ctypes.POINTER(ApplyGradArgs), c_vp, c_i64,
                                                    c_vp]
+    L.ssa_page_plan.restype = ctypes.c_int
+    L.ssa_page_plan.argtypes = [ctypes.POINTER(PagePlanArgs), c_vp]
+    L.ssa_cache_append.restype = ctypes.c_int
+    L.ssa_cache_append.argtypes = [ctypes.POINTER(CacheAppendArgs), c_vp]
+    L.ssa_select_pages.restype = ctypes.c_int
+    L.ssa_select_pages.argtypes = [ctypes.POINTER(SelectPagesArgs), c_vp]
+    L.ssa_cached_attention_workspace_bytes.restype = c_i64
+    L.ssa_cached_attention_workspace_bytes.argtypes = [ctypes.POINTER(CachedAttentionArgs)]
+    L.ssa_cached_attention.restype = ctypes.c_int
+    L.ssa_cached_attention.argtypes = [ctypes.POINTER(CachedAttentionArgs), c_vp, c_i64, c_vp]
     L.ssa_checked_oob.restype = ctypes.c_int
     L.ssa_checked_oob.argtypes = [ctypes.POINTER(ctypes.c_uint32)]
     return L

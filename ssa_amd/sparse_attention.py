@@ -30,6 +30,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
+from .kv_cache import PagedKVCache, PagePlan, cache_append, cached_attention, select_pages
 
 
 # ---------------------------------------------------------------------------- config
@@ -498,6 +499,50 @@ class SparseAttention(nn.Module):
             "padding_fraction": pad if _defer_stats else pad.value(),
         }
 
+    # -------------------------------------------------------------- serving
+    def new_cache(self, num_pages: int, page_size: int = 64) -> PagedKVCache:
+        """An empty paged 8-bit cache for this layer, on its weights' device."""
+        return PagedKVCache(num_pages, self.n_kv, self.d_head, page_size,
+                            device=self.Wk.weight.device)
+
+    def page_budget(self, page_size: int) -> Tuple[int, int, int]:
+        """(top_k, first, recent) for select_pages: as many pages as hold
+        num_neighbors keys, of them always those with the first
+        num_global_tokens tokens and those the window reaches, and room for one
+        other at least."""
+        if self.config.global_token_indices is not None:
+            raise ValueError("page selection takes num_global_tokens; explicit "
+                             "global_token_indices have no counterpart in it")
+        first = -(-self.config.num_global_tokens // page_size)
+        recent = 1 + -(-self.config.window_size // page_size)
+        return max(-(-self.K // page_size), first + recent + 1), first, recent
+
+    def forward_cached(self, x: torch.Tensor, cache: PagedKVCache, plan: PagePlan, *,
+                       sparse: bool = True) -> torch.Tensor:
+        """Attention output (T, d_model) for the new rows x (T, d_model) of a
+        batch of cached sequences (no counterpart in the reference): their keys
+        and values are appended to `cache`, then each row attends to its
+        sequence's cached keys up to itself: those of page_budget()'s pages, or
+        all of them where `sparse` is False.  Causal, inference only, without
+        dropout."""
+        if not self.config.causal:
+            raise ValueError("forward_cached needs config.causal=True: a cached token is not "
+                             "computed again when later ones arrive")
+        if x.dim() != 2:
+            raise ValueError(f"forward_cached takes packed rows (T, d_model), got "
+                             f"{tuple(x.shape)}")
+        budget = self.page_budget(cache.page_size) if sparse else None
+        T = x.shape[0]
+        q = self.Wq(x).view(T, self.H, self.d_head)
+        kv = F.linear(x, self._fused_weight((self.Wk, self.Wv))).view(T, 2 * self.n_kv,
+                                                                     self.d_head)
+        cache_append(cache, kv[:, :self.n_kv], kv[:, self.n_kv:], plan.slots)
+        pages = None
+        if budget is not None:
+            pages = select_pages(q, cache, plan, budget[0], first=budget[1], recent=budget[2])
+        out = cached_attention(q, cache, plan, scale=self.scale, pages=pages)
+        return self.Wo(out.view(T, self.H * self.d_head))
+
 
 class _PendingFraction:
     """Mean of a boolean mask as the reference's CPU ``.float().mean()``
@@ -551,6 +596,11 @@ class SparseTransformerLayer(nn.Module):
         h = x + a
         return h + self.ff(self.norm2(h)), stats
 
+    def forward_cached(self, x, cache: PagedKVCache, plan: PagePlan, *, sparse: bool = True):
+        """The block for the new rows x (T, d_model) of cached sequences."""
+        h = x + self.attn.forward_cached(self.norm1(x), cache, plan, sparse=sparse)
+        return h + self.ff(self.norm2(h))
+
 
 class SparseTransformer(nn.Module):
     """Optional embedding, a stack of SparseTransformerLayer, final LayerNorm
@@ -570,6 +620,22 @@ class SparseTransformer(nn.Module):
             x, stats = layer(x, return_stats=return_stats, _defer_stats=True)
             stats_list.append(stats)
         return self.norm(x), _resolve_stats(stats_list)
+
+    def new_caches(self, num_pages: int, page_size: int = 64) -> list:
+        """An empty cache for every layer; they share block tables."""
+        return [layer.attn.new_cache(num_pages, page_size) for layer in self.layers]
+
+    def forward_cached(self, x, caches, plan: PagePlan, *, sparse: bool = True):
+        """Hidden states (T, d_model) for the new rows of cached sequences: x
+        (T,) token ids or (T, d_model), their place from PageTable.plan.  Rows
+        of padding or of a refused sequence hold values of no meaning."""
+        if len(caches) != len(self.layers):
+            raise ValueError(f"{len(caches)} caches for {len(self.layers)} layers")
+        if self.embed is not None:
+            x = self.embed(x)
+        for layer, cache in zip(self.layers, caches):
+            x = layer.forward_cached(x, cache, plan, sparse=sparse)
+        return self.norm(x)
 
 
 # ---------------------------------------------------------------------------- graph reuse
