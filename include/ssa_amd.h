@@ -405,8 +405,8 @@ int ssa_select_pages(const ssa_select_pages_args *a, void *stream);
  * positions[t] of the row's request, all of them or those of `pages` (T, Hkv, top;
  * negative: none; each page at most once).  q and out (T, Hq, d), unit last
  * strides; out in q's type.  Query head g reads kv head g / (Hq / Hkv).  Products
- * of q and codes are exact, sums and softmax in fp32, probabilities to 16 bits
- * (24 for fp32 q).  A row that sees no key gets zeros.  Needs a 16-byte aligned
+ * of q and codes are exact, sums and softmax in fp32, probabilities to 11 bits or
+ * more (24 for fp32 q).  A row that sees no key gets zeros.  Needs a 16-byte aligned
  * workspace of ssa_cached_attention_workspace_bytes (0 for some sizes). */
 typedef struct {
     ssa_kv_cache cache;

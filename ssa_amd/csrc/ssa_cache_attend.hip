@@ -18,103 +18,29 @@
 // scale is a power of two.  q and p are split into bf16 terms whose sum has the
 // precision that is wanted (bf16 q 1 term, fp16 2, fp32 3; p 2 or 3), so every
 // product is exact and only fp32 sums round.
-#include "ssa_cache_dev.h"
+#include "ssa_cache_attend_dev.h"
 
 namespace {
-
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-typedef __attribute__((ext_vector_type(4))) float f32x4;
-
-constexpr int WAVES = 4;                      // of a workgroup
-constexpr float LOG2E = 1.44269504088896340736f;
-
-struct AttendParams {
-    const uint8_t *k, *v;
-    const float *ks, *vs;
-    const int32_t *table, *starts, *requests, *positions, *pages;
-    const void *q;
-    void *out;
-    float *part_ml, *part_o;                  // (T * Hq, S, 2), (T * Hq, S, D)
-    int64_t num_pages, table_stride, q_st, q_sh, o_st, o_sh;
-    int32_t T, R, width, Hq, Hkv, rep, d, page_shift, top, S, chunk;
-    float scale;                              // softmax scale * log2(e)
-};
-
-__device__ __forceinline__ bf16x8 zero8() {
-    bf16x8 z;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) z[j] = (__bf16)0.f;
-    return z;
-}
-
-// eight codes (two words) as bf16 times scale
-__device__ __forceinline__ bf16x8 codes_bf16(uint32_t w0, uint32_t w1, float scale) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
-    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false);
-    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
-    bf16x8 r;
-    r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1];
-    r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
-    return r;
-}
-
-__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-// the request whose units hold unit u, where request r (R stands for the rows
-// behind the last one) has its units from floor(starts[r] rep / CT) + r on: these
-// leave each request ceil(rows rep / CT) and need no list
-__device__ __forceinline__ int unit_request(const AttendParams &p, int u, int CT) {
-    int lo = 0, hi = p.R;                     // last r with base(r) <= u
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        const int64_t base = (int64_t)p.starts[mid] * p.rep / CT + mid;
-        if (base <= u) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
 
 // A workgroup takes 16 RT columns (query rows of one request and kv head) and a
 // chunk of the key tiles; its waves take every fourth tile of the chunk.
 template <typename T, int D, int KT, int RT>
-__global__ void __launch_bounds__(WAVES * SSA_WAVE)
+__global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE)
 cache_attend_kernel(AttendParams p) {
     constexpr int NQ = sizeof(T) == 4 ? 3 : (__is_same(T, f16_t) ? 2 : 1);
     constexpr int NP = sizeof(T) == 4 ? 3 : 2;
     constexpr int CT = 16 * RT, NB = KT / 16, DP = D / 64, ND = D / 16, KS = KT / 32;
     constexpr int OS = D + 4;                 // row stride of the waves' sums in LDS
     __shared__ float o_lds[CT * OS];
-    __shared__ float m_lds[WAVES][CT], l_lds[WAVES][CT];
+    __shared__ float m_lds[ATT_WAVES][CT], l_lds[ATT_WAVES][CT];
 
     const int lane = lane_id(), col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / SSA_WAVE);
     const int h = (int)blockIdx.y, split = (int)blockIdx.z;
 
-    // this unit's columns: row t0 + c / rep, head c % rep, for c in [c0, c1)
-    int req, t0, c0, c1;
-    if (p.pages) {
-        const int tiles = (p.rep + CT - 1) / CT;
-        t0 = (int)blockIdx.x / tiles;
-        c0 = ((int)blockIdx.x - t0 * tiles) * CT;
-        c1 = min(c0 + CT, p.rep);
-        req = p.requests[t0];
-    } else {
-        const int u = (int)blockIdx.x;
-        const int r = unit_request(p, u, CT);
-        t0 = p.starts[r];
-        const int end = r < p.R ? p.starts[r + 1] : p.T;
-        const int64_t j = u - ((int64_t)t0 * p.rep / CT + r);
-        const int64_t cols = (int64_t)(min(end, p.T) - t0) * p.rep;
-        if (t0 < 0 || j < 0 || j * CT >= cols) return;   // no such unit
-        c0 = (int)(j * CT);
-        c1 = (int)min((int64_t)c0 + CT, cols);
-        req = r < p.R ? r : -1;
-    }
-    if (req >= p.R) req = -1;
+    Unit un;
+    if (!locate_unit(p, (int)blockIdx.x, CT, un)) return;
+    const int req = un.req, t0 = un.t0, c0 = un.c0, c1 = un.c1;
 
     int pos[RT];                              // last key each column sees
     int64_t qrow[RT];
@@ -153,7 +79,7 @@ cache_attend_kernel(AttendParams p) {
 #pragma unroll
         for (int s = 0; s < DP * 2; ++s)
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) qf[rt][s][n] = zero8();
+            for (int n = 0; n < NQ; ++n) qf[rt][s][n] = bf16x8{};
     }
     if (tile0 < tile1) {
 #pragma unroll
@@ -174,7 +100,7 @@ cache_attend_kernel(AttendParams p) {
     }
 
     const int32_t *table = p.table + (int64_t)(req < 0 ? 0 : req) * p.table_stride;
-    for (int tile = tile0 + wave; tile < tile1; tile += WAVES) {
+    for (int tile = tile0 + wave; tile < tile1; tile += ATT_WAVES) {
         int lp = tile / sub_tiles;
         const int sub = tile - lp * sub_tiles;
         if (list) lp = list[lp];
@@ -276,12 +202,12 @@ cache_attend_kernel(AttendParams p) {
         }
     }
     __syncthreads();
-    for (int w = 0; w < WAVES; ++w) {
+    for (int w = 0; w < ATT_WAVES; ++w) {
         if (w == wave) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 float mx = -INFINITY;
-                for (int v = 0; v < WAVES; ++v) mx = fmaxf(mx, m_lds[v][rt * 16 + col]);
+                for (int v = 0; v < ATT_WAVES; ++v) mx = fmaxf(mx, m_lds[v][rt * 16 + col]);
                 const float a = __builtin_amdgcn_exp2f(m[rt] - (mx == -INFINITY ? 0.f : mx));
 #pragma unroll
                 for (int i = 0; i < ND; ++i) {
@@ -293,13 +219,13 @@ cache_attend_kernel(AttendParams p) {
         }
         __syncthreads();
     }
-    for (int i = (int)threadIdx.x; i < CT * D; i += WAVES * SSA_WAVE) {
+    for (int i = (int)threadIdx.x; i < CT * D; i += ATT_WAVES * SSA_WAVE) {
         const int c = i / D, x = i - c * D;
         if (c0 + c >= c1) break;
         float mx = -INFINITY, sum = 0.f;
-        for (int v = 0; v < WAVES; ++v) mx = fmaxf(mx, m_lds[v][c]);
+        for (int v = 0; v < ATT_WAVES; ++v) mx = fmaxf(mx, m_lds[v][c]);
         const float ms = mx == -INFINITY ? 0.f : mx;
-        for (int v = 0; v < WAVES; ++v)
+        for (int v = 0; v < ATT_WAVES; ++v)
             sum += l_lds[v][c] * __builtin_amdgcn_exp2f(m_lds[v][c] - ms);
         const int t = t0 + (c0 + c) / p.rep, hq = h * p.rep + (c0 + c) % p.rep;
         const float v = o_lds[c * OS + x];
@@ -308,7 +234,7 @@ cache_attend_kernel(AttendParams p) {
                 Cvt<T>::store((T *)p.out + t * p.o_st + hq * p.o_sh + x,
                               sum == 0.f ? 0.f : v / sum);
         } else {
-            const int64_t at = ((int64_t)t * p.Hq + hq) * p.S + split;
+            const int64_t at = ((int64_t)t * p.Hq + hq) * p.s_stride + split;
             if (tile0 < tile1) p.part_o[at * D + x] = v;
             if (x == 0) {
                 p.part_ml[2 * at] = mx;
@@ -318,29 +244,45 @@ cache_attend_kernel(AttendParams p) {
     }
 }
 
-// Joins the S chunks of each query row: one wave per row.  Bound by latency.
+// Joins the S chunks of each column: one wave per column.  Bound by latency, so the
+// chunks' weights are formed side by side, a lane each.
 template <typename T, int D>
-__global__ void __launch_bounds__(WAVES * SSA_WAVE)
-cache_join_kernel(AttendParams p) {
-    const int64_t row = (int64_t)blockIdx.x * WAVES + threadIdx.x / SSA_WAVE;
-    if (row >= (int64_t)p.T * p.Hq) return;
+__global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE)
+cache_join_kernel(AttendParams p, int CT) {
+    Unit un;
+    if (!locate_unit(p, (int)blockIdx.x, CT, un)) return;
+    const int c = un.c0 + (int)blockIdx.z * ATT_WAVES + (int)threadIdx.x / SSA_WAVE;
+    if (c >= un.c1) return;
     const int lane = lane_id();
+    const int t = un.t0 + c / p.rep, hq = (int)blockIdx.y * p.rep + c % p.rep;
+    const int64_t row = ((int64_t)t * p.Hq + hq) * p.s_stride;
     float mx = -INFINITY;
-    for (int s = 0; s < p.S; ++s) mx = fmaxf(mx, p.part_ml[2 * (row * p.S + s)]);
+    for (int s = lane; s < p.S; s += SSA_WAVE) mx = fmaxf(mx, p.part_ml[2 * (row + s)]);
+    mx = wave_max(mx);
     const float ms = mx == -INFINITY ? 0.f : mx;
     float sum = 0.f, o[D / 64];
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) o[j] = 0.f;
-    for (int s = 0; s < p.S; ++s) {
-        const int64_t at = row * p.S + s;
-        const float m = p.part_ml[2 * at], l = p.part_ml[2 * at + 1];
-        if (l == 0.f) continue;               // nothing seen there (a NaN is not skipped)
-        const float a = __builtin_amdgcn_exp2f(m - ms);
-        sum += l * a;
+    for (int s0 = 0; s0 < p.S; s0 += SSA_WAVE) {
+        const int s = s0 + lane;
+        float w = 0.f, l = 0.f;
+        if (s < p.S) {
+            l = p.part_ml[2 * (row + s) + 1];
+            w = __builtin_amdgcn_exp2f(p.part_ml[2 * (row + s)] - ms);
+        }
+        sum += l * w;
+        // a chunk that saw nothing (l = 0) has written no sums; a NaN is not skipped
+        uint64_t some = wave_ballot(l != 0.f);
+        while (some) {
+            const int i = __ffsll((unsigned long long)some) - 1;
+            some &= some - 1;
+            const float wi = __shfl(w, i, SSA_WAVE);
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) o[j] += p.part_o[at * D + j * 64 + lane] * a;
+            for (int j = 0; j < D / 64; ++j)
+                o[j] += p.part_o[(row + s0 + i) * D + j * 64 + lane] * wi;
+        }
     }
-    const int t = (int)(row / p.Hq), hq = (int)(row - (int64_t)t * p.Hq);
+    sum = wave_sum(sum);
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
         const int x = j * 64 + lane;
@@ -349,36 +291,63 @@ cache_join_kernel(AttendParams p) {
     }
 }
 
-// What a call launches: columns per workgroup, workgroups over the columns, and
-// the chunks that the key tiles are cut into.
+// What a call launches.  A request with more than MANY columns (rows times query
+// heads of a kv head) shares its keys among that many matrix columns, enough for
+// the kernel that stages key tiles in LDS (ssa_cache_prompt.hip); the others are
+// bound by reading keys and go to the kernel above.  The lengths are on the GPU,
+// so the host goes by T / R alone: at most 4 rows a request on average, all go
+// one way (one launch); else both kernels are launched and each leaves the
+// other's requests.
+constexpr int MANY = 64;
+
 struct AttendShape {
-    int RT, KT, S, chunk;
+    int RT, KT, S, chunk;                     // of the kernel above
+    int mode;
     int64_t units;
+    bool prompt;
+    int prompt_S, prompt_chunk, prompt_cols;
+    int64_t prompt_units;
+    int s_stride;
 };
 
+// chunks of the key tiles: about `wgs` workgroups in all, `least` tiles or more each
+void split_tiles(int64_t tiles, int64_t units, int64_t wgs, int least, int *S, int *chunk) {
+    const int64_t want = ceil_div(wgs, units);
+    int64_t c = ceil_div(tiles, want < 1 ? 1 : want);
+    if (c < least) c = least;
+    *S = (int)ceil_div(tiles, c);
+    if (*S < 1) *S = 1;
+    *chunk = (int)c;
+}
+
 AttendShape attend_shape(const ssa_cached_attention_args *a) {
-    AttendShape s;
+    AttendShape s = {};
     const ssa_kv_cache &c = a->cache;
+    const int64_t T = a->rows.T, R = a->rows.R;
     const int rep = a->Hq / c.Hkv;
     s.KT = c.page < 64 ? 32 : 64;
     s.RT = rep > 16 ? 2 : 1;
     const int CT = 16 * s.RT;
     const int per_page = c.page / s.KT;
-    int64_t tiles;                            // the most that a unit can have
+    int64_t tiles = (int64_t)a->rows.width * per_page;   // the most that a unit can have
     if (a->pages) {
-        s.units = (int64_t)a->rows.T * ceil_div(rep, CT);
+        s.mode = UNITS_PAGES;
+        s.units = T * ceil_div(rep, CT);
         tiles = (int64_t)a->top * per_page;
+    } else if (T <= 4 * R || T * rep <= MANY) {
+        s.mode = UNITS_ALL;
+        s.units = T * rep / CT + R + 1;
     } else {
-        s.units = (int64_t)a->rows.T * rep / CT + a->rows.R + 1;
-        tiles = (int64_t)a->rows.width * per_page;
+        s.mode = UNITS_FEW;
+        s.units = (R + 1) * ceil_div(MANY, CT);
+        s.prompt = true;
+        s.prompt_cols = ssa_cache_prompt_columns(a->dtype, c.D);
+        s.prompt_units = T * rep / s.prompt_cols + R + 1;
+        split_tiles(tiles, s.prompt_units * c.Hkv, 512, 16, &s.prompt_S, &s.prompt_chunk);
     }
-    // about 2,048 workgroups, with two tiles or more for each wave
-    const int64_t want = ceil_div(2048, s.units * c.Hkv);
-    int64_t chunk = ceil_div(tiles, want < 1 ? 1 : want);
-    if (chunk < 2 * WAVES) chunk = 2 * WAVES;
-    s.S = (int)ceil_div(tiles, chunk);
-    if (s.S < 1) s.S = 1;
-    s.chunk = (int)chunk;
+    // two tiles or more for each wave
+    split_tiles(tiles, s.units * c.Hkv, 2048, 2 * ATT_WAVES, &s.S, &s.chunk);
+    s.s_stride = s.prompt && s.prompt_S > s.S ? s.prompt_S : s.S;
     return s;
 }
 
@@ -400,13 +369,28 @@ int check_attend(const ssa_cached_attention_args *a) {
     return SSA_OK;
 }
 
+template <typename T, int D>
+void launch_join(AttendParams p, int CT, hipStream_t st) {
+    if (p.S == 1) return;
+    const dim3 grid((unsigned)p.units, (unsigned)p.Hkv, (unsigned)ceil_div(CT, ATT_WAVES));
+    cache_join_kernel<T, D><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p, CT);
+}
+
 template <typename T, int D, int KT, int RT>
 void launch_attend(const AttendParams &p, const AttendShape &s, hipStream_t st) {
-    const dim3 grid((unsigned)s.units, (unsigned)p.Hkv, (unsigned)s.S);
-    cache_attend_kernel<T, D, KT, RT><<<grid, WAVES * SSA_WAVE, 0, st>>>(p);
-    if (s.S > 1)
-        cache_join_kernel<T, D><<<(unsigned)ceil_div((int64_t)p.T * p.Hq, WAVES),
-                                  WAVES * SSA_WAVE, 0, st>>>(p);
+    const dim3 grid((unsigned)p.units, (unsigned)p.Hkv, (unsigned)p.S);
+    cache_attend_kernel<T, D, KT, RT><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
+    launch_join<T, D>(p, 16 * RT, st);
+    if (s.prompt) {
+        AttendParams pp = p;
+        pp.mode = UNITS_MANY;
+        pp.units = (int32_t)s.prompt_units;
+        pp.S = s.prompt_S;
+        pp.chunk = s.prompt_chunk;
+        ssa_cache_prompt_launch(pp, sizeof(T) == 4 ? SSA_F32 : (__is_same(T, f16_t) ? SSA_F16 : SSA_BF16),
+                                D, KT, st);
+        launch_join<T, D>(pp, s.prompt_cols, st);
+    }
 }
 
 template <typename T, int D>
@@ -434,8 +418,8 @@ extern "C" int64_t ssa_cached_attention_workspace_bytes(const ssa_cached_attenti
     if (rc != SSA_OK) return rc;
     if (a->rows.T == 0) return 0;
     const AttendShape s = attend_shape(a);
-    if (s.S == 1) return 0;
-    return (int64_t)a->rows.T * a->Hq * s.S * (2 + a->cache.D) * 4;
+    if (s.s_stride == 1) return 0;
+    return (int64_t)a->rows.T * a->Hq * s.s_stride * (2 + a->cache.D) * 4;
 }
 
 extern "C" int ssa_cached_attention(const ssa_cached_attention_args *a, void *workspace,
@@ -451,7 +435,9 @@ extern "C" int ssa_cached_attention(const ssa_cached_attention_args *a, void *wo
     }
     SSA_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "cached_attention: workspace alignment");
     const AttendShape s = attend_shape(a);
-    SSA_CHECK_ARG(s.units < (1ll << 31) && s.S <= 65535, "cached_attention: too many rows");
+    SSA_CHECK_ARG(s.units < (1ll << 31) && s.S <= 65535 &&
+                      s.prompt_units * a->cache.Hkv < (1ll << 31) && s.prompt_S <= 65535,
+                  "cached_attention: too many rows");
     const ssa_kv_cache &c = a->cache;
     AttendParams p = {};
     p.k = (const uint8_t *)c.k_codes;
@@ -466,7 +452,7 @@ extern "C" int ssa_cached_attention(const ssa_cached_attention_args *a, void *wo
     p.q = a->q;
     p.out = a->out;
     p.part_ml = (float *)workspace;
-    p.part_o = p.part_ml + (int64_t)a->rows.T * a->Hq * s.S * 2;
+    p.part_o = p.part_ml + (int64_t)a->rows.T * a->Hq * s.s_stride * 2;
     p.num_pages = c.num_pages;
     p.table_stride = a->rows.table_stride;
     p.q_st = a->q_st;
@@ -483,6 +469,10 @@ extern "C" int ssa_cached_attention(const ssa_cached_attention_args *a, void *wo
     p.page_shift = c.page == 32 ? 5 : (c.page == 64 ? 6 : 7);
     p.top = a->top;
     p.S = s.S;
+    p.s_stride = s.s_stride;
+    p.mode = s.mode;
+    p.many = MANY;
+    p.units = (int32_t)s.units;
     p.chunk = s.chunk;
     p.scale = a->scale * LOG2E;
     const hipStream_t st = (hipStream_t)stream;

@@ -165,14 +165,15 @@ def select(q, c, table, requests, positions, top, first, recent):
 
 
 def attend(q, c, table, requests, positions, scale, pages=None):
-    """(out, spread, reach): the attention, sum_j p_j |v_j| per element, and per
-    row the largest scale * sum |q| |k| of a key it sees."""
+    """(out, spread, reach, size): the attention, sum_j p_j |v_j| per element, and
+    per row the largest scale * sum |q| |k| and the largest |v| of a key it sees."""
     T, Hq, d = q.shape
     P, H = c.k_scale.shape
     rep = Hq // H
     q = q.cpu().double()
     out = torch.zeros(T, Hq, d, dtype=torch.float64)
-    spread, reach = torch.zeros_like(out), torch.zeros(T, Hq, 1, dtype=torch.float64)
+    spread = torch.zeros_like(out)
+    reach, size = (torch.zeros(T, Hq, 1, dtype=torch.float64) for _ in range(2))
     for t in range(T):
         r, pos = requests[t], positions[t]
         if r < 0 or r >= len(table) or pos < 0:
@@ -195,21 +196,26 @@ def attend(q, c, table, requests, positions, scale, pages=None):
             s = q[t, g] @ k.T * scale
             p = torch.softmax(s, 1)
             out[t, g], spread[t, g] = p @ v, p @ v.abs()
-            reach[t, g, 0] = (q[t, g].abs() @ k.abs().T).amax(1) * scale
-    return out, spread, reach
+            reach[t, g, 0] = (q[t, g].abs() @ k.abs().T).amax(1) * abs(scale)
+            size[t, g, 0] = v.abs().max()
+    return out, spread, reach, size
 
 
-def attend_tolerance(out, spread, reach, dtype, keys, d):
+def attend_tolerance(out, spread, reach, size, dtype, keys, d):
     """How far a result may be from `out`, per element.
 
-    The result is rounded to its type once: finfo.eps / 2 of its value.  The
-    probabilities are sums of two bf16 terms, off by 2^-16 of their value (three
-    for fp32 queries: 2^-24).  Products are exact; a score is a sum of d terms in
-    fp32, off by (d + 2) 2^-24 of its terms' magnitudes (2^-23 where a step
-    truncates), which enters the exponential, the sum and the maximum: twice.  The
-    exponential is off by 2^-22; the sums over the keys by keys * 2^-23 each, the
-    numerator's and the denominator's."""
+    The result is rounded to its type once: finfo.eps / 2 of its value.  A
+    probability p is rounded to f16 (fp32 queries: to three bf16 terms, 24 bits):
+    off by 2^-11 of its value (2^-24), and where that f16 is subnormal by half its
+    step, 2^-25: 2^-30 of the largest p, which is kept 2^5 above 1.  The numerator
+    sum p v has these errors times |v|, the denominator sum p >= 1 those of the
+    same rounded p, and the quotient is at most spread / 1: twice 2^-11 spread, and
+    twice keys * 2^-30 * the largest |v|.  Products are exact; a score is a sum of
+    d terms in fp32, off by (d + 2) 2^-24 of its terms' magnitudes (2^-23 where a
+    step truncates), which enters the exponential, the sum and the maximum: twice.
+    The exponential is off by 2^-22; the sums over the keys by keys * 2^-23 each,
+    the numerator's and the denominator's."""
     half = torch.finfo(dtype).eps / 2
-    term = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -16
+    term, least = (2.0 ** -24, 0.0) if dtype == torch.float32 else (2 * 2.0 ** -11, 2.0 ** -29)
     rel = term + 2 * (d + 2) * 2.0 ** -23 * reach + 2.0 ** -21 + 2 * keys * 2.0 ** -23
-    return half * out.abs() + rel * (1 + half) * spread + 2.0 ** -120
+    return half * out.abs() + (1 + half) * (rel * spread + least * keys * size) + 2.0 ** -120

@@ -306,11 +306,11 @@ def _check_attend(c, b, q, qd, *, pages=None, scale=None, out=None):
     d = q.shape[2]
     got = ssa_amd.cached_attention(qd, c, _plan(b), scale=scale, out=out,
                                    pages=None if pages is None else pages.to(DEV))
-    want, spread, reach = ref.attend(q, ref.Cache.of(c), b[0], b[2], b[3],
+    want, *sizes = ref.attend(q, ref.Cache.of(c), b[0], b[2], b[3],
                                      d ** -0.5 if scale is None else scale, pages)
     assert got.dtype == q.dtype and got.shape == q.shape
     keys = max(b[3] + [0]) + 1
-    tol = ref.attend_tolerance(want, spread, reach, q.dtype, keys, d)
+    tol = ref.attend_tolerance(want, *sizes, q.dtype, keys, d)
     x = got.cpu().double()
     assert torch.equal(x.isnan(), want.isnan())
     ok = ((x - want).abs() <= tol) | want.isnan()
@@ -462,8 +462,8 @@ def test_offsets_beyond_32_bits():
                             _i32([148, 149]))
     q = torch.randn(2, 16, d, generator=g)
     got = ssa_amd.cached_attention(q.to(DEV), c, plan).cpu().double()
-    want, spread, reach = ref.attend(q, small, [[0, 1, 2]], [0, 0], [148, 149], d ** -0.5)
-    tol = ref.attend_tolerance(want, spread, reach, F32, 150, d)
+    want, *sizes = ref.attend(q, small, [[0, 1, 2]], [0, 0], [148, 149], d ** -0.5)
+    tol = ref.attend_tolerance(want, *sizes, F32, 150, d)
     assert bool(((got - want).abs() <= tol).all())
     got = ssa_amd.select_pages(q.to(DEV), c, plan, 2).cpu()
     assert torch.equal(got, ref.select(q, small, [[0, 1, 2]], [0, 0], [148, 149], 2, 1, 1))
@@ -500,8 +500,8 @@ def test_layer_over_cached_tokens(sparse):
         if sparse:
             top, first, recent = attn.page_budget(ps)
             pages = ref.select(q, c, *rows, top, first, recent)
-        want, spread, reach = ref.attend(q, c, *rows, attn.scale, pages)
-        tol = ref.attend_tolerance(want, spread, reach, F32, max(lengths), d)
+        want, *sizes = ref.attend(q, c, *rows, attn.scale, pages)
+        tol = ref.attend_tolerance(want, *sizes, F32, max(lengths), d)
         W = attn.Wo.weight.double().cpu()
         want, tol = want.reshape(T, -1), tol.reshape(T, -1)
         # the output projection: H d products and sums in fp32
