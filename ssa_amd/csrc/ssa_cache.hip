@@ -127,13 +127,37 @@ page_plan_kernel(ssa_page_plan_args a) {
 // One workgroup per run of adjacent rows of one page and kv head: the run's
 // largest magnitudes first (the page's scale has to hold before any code is
 // rounded), then the codes, staged in LDS so that the transposed value codes go
-// out in words of four tokens.  Reads every row twice, the second time from the
-// L2.  Bound by latency for single tokens, by HBM for prompts.
+// out 16 tokens at a time.  D / 8 lanes hold a row, 8 columns each; every row is
+// read twice, the second time from the L2.  Bound by latency for single tokens
+// (about five dependent steps), by reading and writing HBM for prompts.
 constexpr int APP_THREADS = 256;
 
-template <typename T>
-__device__ __forceinline__ float row_elem(const void *p, int64_t i) {
-    return to_f32(((const T *)p)[i]);
+// columns x .. x + 7 of a row, zeros past d.  VEC: d and the strides are multiples
+// of 8 (the addresses of 16 bytes)
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_row8(const void *p, int64_t at, int x, int d, float (&v)[8]) {
+    const T *q = (const T *)p + at + x;
+    if (VEC) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        if (x < d) {
+            T t[8];
+            __builtin_memcpy(t, __builtin_assume_aligned(q, 16), sizeof(t));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = to_f32(t[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = x + j < d ? to_f32(q[j]) : 0.f;
+    }
+}
+
+// bits of the largest magnitude; a NaN's, its sign cleared, pass every number's
+__device__ __forceinline__ uint32_t max_bits8(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+    return m;
 }
 
 // smallest e with a <= 448 * 2^e: 448 = 1.75 * 2^8
@@ -146,46 +170,83 @@ __device__ __forceinline__ float exp2_int(int e) {      // -126 <= e <= 127
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-template <typename T>
+// a code's place in the order of the numbers (-126..126; NaN is told apart before)
+__device__ __forceinline__ int code_rank(uint32_t code) {
+    return (code & 0x80u) ? -(int)(code & 0x7fu) : (int)(code & 0x7fu);
+}
+
+template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(APP_THREADS)
 cache_append_kernel(ssa_cache_append_args a, int window) {
+    constexpr int LPR = D / 8, RPW = APP_THREADS / LPR;   // lanes of a row, rows at a time
     extern __shared__ uint4 app_lds[];
     __shared__ uint32_t kmax[128], vmax[128];     // bits of each row's largest magnitude
     __shared__ uint32_t page_max[2], any_bad;
+    __shared__ int lo_lds[D], hi_lds[D];
     const ssa_kv_cache &c = a.cache;
-    const int h = (int)blockIdx.y, ps = c.page, D = c.D, d = c.d, tid = (int)threadIdx.x;
+    const int h = (int)blockIdx.y, ps = c.page, d = c.d, tid = (int)threadIdx.x;
+    const int lane = lane_id(), rx = tid % LPR * 8, r0 = tid / LPR;
     const int64_t cap = c.num_pages * ps;
     uint8_t *kst = (uint8_t *)app_lds, *vst = kst + ps * D;      // [row][D] codes
-    for (int w = 0; w < window; ++w) {
-        const int64_t t0 = (int64_t)blockIdx.x * window + w;
-        if (t0 >= a.T) break;
-        const int64_t slot = a.slots[t0];
-        if (slot < 0 || slot >= cap) continue;
+
+    // the window's first rows of runs: every wave finds them for itself
+    const int64_t w0 = (int64_t)blockIdx.x * window;
+    int64_t mine = -1;
+    bool first = false;
+    if (lane < window && w0 + lane < a.T) {
+        mine = a.slots[w0 + lane];
+        const int64_t prev = w0 + lane > 0 ? a.slots[w0 + lane - 1] : -1;
+        first = mine >= 0 && mine < cap && (mine % ps == 0 || prev != mine - 1);
+    }
+    uint64_t todo = wave_ballot(first);
+    while (todo) {
+        const int w = __ffsll((unsigned long long)todo) - 1;
+        todo &= todo - 1;
+        const int64_t t0 = w0 + w, slot = __shfl(mine, w, SSA_WAVE);
         const int64_t pg = slot / ps;
         const int off = (int)(slot - pg * ps);
-        if (off != 0 && t0 > 0 && a.slots[t0 - 1] == slot - 1) continue;   // inside a run
         // length of the run: rows t0 + i at slot + i within the page
         const int most = (int)min((int64_t)(ps - off), a.T - t0);
         int n = 1;
         for (int b = 0; b < most; b += SSA_WAVE) {
-            const int i = b + lane_id();
+            const int i = b + lane;
             const uint64_t m = wave_ballot(i < most && a.slots[t0 + i] == slot + i);
             n = b + (m == ~0ull ? SSA_WAVE : __ffsll((unsigned long long)~m) - 1);
             if (m != ~0ull) break;
         }
-        n = min(n, most);
-        __syncthreads();                                   // the last run's LDS is read
-        if (tid < 128) kmax[tid] = vmax[tid] = 0;
-        if (tid < 2) page_max[tid] = 0;
-        if (tid == 2) any_bad = 0;
-        __syncthreads();
+        const int64_t ph = pg * c.Hkv + h;
+        const float k_old = off ? c.k_scale[ph] : 0.f, v_old = off ? c.v_scale[ph] : 0.f;
         const int64_t krow = t0 * a.k_st + (int64_t)h * a.k_sh;
         const int64_t vrow = t0 * a.v_st + (int64_t)h * a.v_sh;
-        for (int i = tid; i < n * d; i += APP_THREADS) {
-            const int r = i / d, x = i - r * d;
-            // a NaN's bits, its sign cleared, are larger than every number's
-            atomicMax(&kmax[r], __float_as_uint(row_elem<T>(a.k, krow + r * a.k_st + x)) & 0x7fffffffu);
-            atomicMax(&vmax[r], __float_as_uint(row_elem<T>(a.v, vrow + r * a.v_st + x)) & 0x7fffffffu);
+        __syncthreads();                                   // the last run's LDS is read
+        if (tid < 2) page_max[tid] = 0;
+        if (tid == 2) any_bad = 0;
+        for (int b = r0; b - r0 < n; b += 4 * RPW) {       // four rows in flight
+            uint32_t km[4], vm[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = b + i * RPW;
+                float kv[8] = {}, vv[8] = {};
+                if (r < n) {
+                    load_row8<T, VEC>(a.k, krow + r * a.k_st, rx, d, kv);
+                    load_row8<T, VEC>(a.v, vrow + r * a.v_st, rx, d, vv);
+                }
+                km[i] = max_bits8(kv);
+                vm[i] = max_bits8(vv);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) {
+                    km[i] = max(km[i], (uint32_t)__shfl_xor((int)km[i], o, SSA_WAVE));
+                    vm[i] = max(vm[i], (uint32_t)__shfl_xor((int)vm[i], o, SSA_WAVE));
+                }
+                const int r = b + i * RPW;
+                if (rx == 0 && r < n) {
+                    kmax[r] = km[i];
+                    vmax[r] = vm[i];
+                }
+            }
         }
         __syncthreads();
         if (tid < n) {
@@ -199,8 +260,6 @@ cache_append_kernel(ssa_cache_append_args a, int window) {
             }
         }
         __syncthreads();
-        const int64_t ph = pg * c.Hkv + h;
-        const float k_old = off ? c.k_scale[ph] : 0.f, v_old = off ? c.v_scale[ph] : 0.f;
         const float k_new = fmaxf(k_old, exp2_int(scale_exponent(__uint_as_float(page_max[0]))));
         const float v_new = fmaxf(v_old, exp2_int(scale_exponent(__uint_as_float(page_max[1]))));
         uint8_t *kp = (uint8_t *)c.k_codes + ph * ps * D, *vp = (uint8_t *)c.v_codes + ph * D * ps;
@@ -213,75 +272,118 @@ cache_append_kernel(ssa_cache_append_args a, int window) {
         if (v_old < v_new && off) {
             const float f = v_old / v_new;
             uint32_t *p = (uint32_t *)vp;
-            const int words = (off + 3) / 4;               // of each channel's tokens
+            const int words = ps / 4;                      // of each channel's tokens
             for (int i = tid; i < D * words; i += APP_THREADS) {
-                const int x = i / words, q = i - x * words;
-                uint32_t *at = p + x * (ps / 4) + q;
-                const uint32_t was = *at, now = codes4_scaled(was, f);
-                const int keep = min(off - 4 * q, 4) * 8;  // bits of tokens below the run
-                const uint32_t m = keep == 32 ? ~0u : (1u << keep) - 1u;
-                *at = (now & m) | (was & ~m);
+                const int keep = off - 4 * (i & (words - 1));   // tokens below the run
+                if (keep <= 0) continue;
+                const uint32_t was = p[i], now = codes4_scaled(was, f);
+                const uint32_t m = keep >= 4 ? ~0u : (1u << 8 * keep) - 1u;
+                p[i] = (now & m) | (was & ~m);
             }
+        }
+        // bounds that stay, at the new scale
+        const bool bad_page = any_bad != 0;
+        for (int x = tid; x < D; x += APP_THREADS) {
+            int lo = 127, hi = -127;
+            if (off) {
+                const float f = k_old / k_new;
+                const uint32_t cd = codes2(code_f32<0>(bp[x]) * f, code_f32<0>(bp[D + x]) * f);
+                const bool nan = (cd & 0x7fu) == SSA_CODE_NAN || ((cd >> 8) & 0x7fu) == SSA_CODE_NAN;
+                lo = nan ? -127 : code_rank(cd & 0xffu);
+                hi = nan ? 127 : code_rank(cd >> 8);
+            }
+            lo_lds[x] = lo;
+            hi_lds[x] = hi;
         }
         const float ki = 1.f / k_new, vi = 1.f / v_new;    // exact
-        for (int i = tid; i < n * (D / 2); i += APP_THREADS) {
-            const int r = i / (D / 2), x = 2 * (i - r * (D / 2));
+#pragma unroll 4
+        for (int r = r0; r < n; r += RPW) {
+            float kv[8], vv[8];
+            load_row8<T, VEC>(a.k, krow + r * a.k_st, rx, d, kv);
+            load_row8<T, VEC>(a.v, vrow + r * a.v_st, rx, d, vv);
             const bool bad = kmax[r] == 0xffffffffu;
-            const int64_t ko = krow + r * a.k_st + x, vo = vrow + r * a.v_st + x;
-            const float k0 = x < d ? row_elem<T>(a.k, ko) : 0.f;
-            const float k1 = x + 1 < d ? row_elem<T>(a.k, ko + 1) : 0.f;
-            const float v0 = x < d ? row_elem<T>(a.v, vo) : 0.f;
-            const float v1 = x + 1 < d ? row_elem<T>(a.v, vo + 1) : 0.f;
-            *(uint16_t *)(kst + r * D + x) =
-                (uint16_t)(bad ? SSA_CODE_NAN * 0x101u : codes2(k0 * ki, k1 * ki));
-            *(uint16_t *)(vst + r * D + x) = (uint16_t)(bad ? 0u : codes2(v0 * vi, v1 * vi));
+            uint2 kc, vc;
+            kc.x = codes4(kv[0] * ki, kv[1] * ki, kv[2] * ki, kv[3] * ki);
+            kc.y = codes4(kv[4] * ki, kv[5] * ki, kv[6] * ki, kv[7] * ki);
+            vc.x = codes4(vv[0] * vi, vv[1] * vi, vv[2] * vi, vv[3] * vi);
+            vc.y = codes4(vv[4] * vi, vv[5] * vi, vv[6] * vi, vv[7] * vi);
+            if (bad) {
+                kc.x = kc.y = SSA_CODE_NAN * 0x01010101u;
+                vc.x = vc.y = 0;
+            }
+            *(uint2 *)(kst + r * D + rx) = kc;
+            *(uint2 *)(vst + r * D + rx) = vc;
+            *(uint2 *)(kp + (int64_t)(off + r) * D + rx) = kc;
         }
         __syncthreads();
-        for (int i = tid; i < n * D / 16; i += APP_THREADS)
-            ((uint4 *)(kp + (int64_t)off * D))[i] = ((const uint4 *)kst)[i];
-        const int q0 = off / 4, q1 = (off + n + 3) / 4;    // words of a channel's tokens
-        for (int i = tid; i < D * (q1 - q0); i += APP_THREADS) {
-            const int x = i % D, q = q0 + i / D;
-            uint32_t v = 0;
-            bool whole = true;
+        // values: 4 columns x 16 tokens at a time, turned in registers
+        const int g0 = off / 16, g1 = (off + n + 15) / 16;
+        for (int i = tid; i < D / 4 * (g1 - g0); i += APP_THREADS) {
+            const int x = i % (D / 4) * 4, tok = (g0 + i / (D / 4)) * 16;
+            if (tok >= off && tok + 16 <= off + n) {
+                uint32_t w[4][4];                          // [column][four tokens]
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = 4 * q + j - off;
-                if (r >= 0 && r < n) v |= (uint32_t)vst[r * D + x] << (8 * j);
-                else whole = false;
-            }
-            uint8_t *at = vp + (int64_t)x * ps + 4 * q;
-            if (whole) {
-                *(uint32_t *)at = v;
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t in[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        in[j] = *(const uint32_t *)(vst + (tok - off + 4 * q + j) * D + x);
+                    // bytes (row, column) -> (column, row)
+                    const uint32_t a0 = __builtin_amdgcn_perm(in[1], in[0], 0x05010400u);
+                    const uint32_t a1 = __builtin_amdgcn_perm(in[1], in[0], 0x07030602u);
+                    const uint32_t b0 = __builtin_amdgcn_perm(in[3], in[2], 0x05010400u);
+                    const uint32_t b1 = __builtin_amdgcn_perm(in[3], in[2], 0x07030602u);
+                    w[0][q] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
+                    w[1][q] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
+                    w[2][q] = __builtin_amdgcn_perm(b1, a1, 0x05040100u);
+                    w[3][q] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *(uint4 *)(vp + (int64_t)(x + j) * ps + tok) =
+                        uint4{w[j][0], w[j][1], w[j][2], w[j][3]};
             } else {
+                const int e = min(tok + 16, off + n);
+                for (int q = max(tok, off); q < e; ++q) {
+                    const uint32_t v = *(const uint32_t *)(vst + (q - off) * D + x);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = 4 * q + j - off;
-                    if (r >= 0 && r < n) at[j] = (uint8_t)(v >> (8 * j));
+                    for (int j = 0; j < 4; ++j) vp[(int64_t)(x + j) * ps + q] = (uint8_t)(v >> 8 * j);
                 }
             }
         }
-        // bounds: a code's order is that of its sign and magnitude
-        for (int x = tid; x < D; x += APP_THREADS) {
-            int lo = 127, hi = -127;
-            bool nan = any_bad != 0;
-            auto note = [&](uint32_t code) {
-                const int v = (code & 0x80u) ? -(int)(code & 0x7fu) : (int)code;
-                nan |= (code & 0x7fu) == SSA_CODE_NAN;
-                lo = min(lo, v);
-                hi = max(hi, v);
-            };
-            if (off) {
-                const float f = k_old / k_new;
-                note(codes2(code_f32<0>(bp[x]) * f, 0.f) & 0xffu);
-                note(codes2(code_f32<0>(bp[D + x]) * f, 0.f) & 0xffu);
+        // bounds: 4 columns and every RB-th row a thread
+        constexpr int RB = APP_THREADS / (D / 4);
+        {
+            const int x = tid % (D / 4) * 4;
+            int lo[4], hi[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                lo[j] = 127;
+                hi[j] = -127;
             }
-            for (int r = 0; r < n; ++r) note(kst[r * D + x]);
-            auto code = [&](int v) {
-                return (uint8_t)(nan ? SSA_CODE_NAN : (v < 0 ? 0x80u | (uint32_t)-v : (uint32_t)v));
-            };
-            bp[x] = code(lo);
-            bp[D + x] = code(hi);
+            for (int r = tid / (D / 4); r < n; r += RB) {
+                const uint32_t v = *(const uint32_t *)(kst + r * D + x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int k = code_rank((v >> 8 * j) & 0xffu);
+                    lo[j] = min(lo[j], k);
+                    hi[j] = max(hi[j], k);
+                }
+            }
+            if (tid / (D / 4) < n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    atomicMin(&lo_lds[x + j], lo[j]);
+                    atomicMax(&hi_lds[x + j], hi[j]);
+                }
+        }
+        __syncthreads();
+        for (int x = tid; x < D; x += APP_THREADS) {
+            const int lo = lo_lds[x], hi = hi_lds[x];
+            const bool nan = bad_page || lo == -127;       // only a NaN bound ranks there
+            auto code = [](int v) { return (uint8_t)(v < 0 ? 0x80 | -v : v); };
+            bp[x] = nan ? (uint8_t)SSA_CODE_NAN : code(lo);
+            bp[D + x] = nan ? (uint8_t)SSA_CODE_NAN : code(hi);
         }
         if (tid == 0) {
             c.k_scale[ph] = k_new;
@@ -290,13 +392,43 @@ cache_append_kernel(ssa_cache_append_args a, int window) {
     }
 }
 
+template <typename T, int D>
+int launch_append(const ssa_cache_append_args &a, hipStream_t s) {
+    // a workgroup looks at `window` rows for the first rows of runs: one each while
+    // every row may be one (single tokens: a run each), more where most lie inside
+    const int window = a.T <= 1024 ? 1 : (a.T <= 4096 ? 4 : 16);
+    const dim3 grid((unsigned)ceil_div(a.T, window), (unsigned)a.cache.Hkv);
+    const size_t lds = (size_t)2 * a.cache.page * D;
+    // rows in 16-byte pieces (8 elements) where they all start at one
+    const int64_t strides = a.k_st | a.k_sh | a.v_st | a.v_sh;
+    const bool vec = a.cache.d % 8 == 0 && (strides * (int64_t)sizeof(T)) % 16 == 0 &&
+                     (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0;
+    if (vec) {
+        SSA_ALLOW_LDS((cache_append_kernel<T, D, true>), lds);
+        cache_append_kernel<T, D, true><<<grid, APP_THREADS, lds, s>>>(a, window);
+    } else {
+        SSA_ALLOW_LDS((cache_append_kernel<T, D, false>), lds);
+        cache_append_kernel<T, D, false><<<grid, APP_THREADS, lds, s>>>(a, window);
+    }
+    return SSA_OK;
+}
+
+template <typename T>
+int launch_append_t(const ssa_cache_append_args &a, hipStream_t s) {
+    return a.cache.D == 64 ? launch_append<T, 64>(a, s)
+                           : (a.cache.D == 128 ? launch_append<T, 128>(a, s)
+                                               : launch_append<T, 256>(a, s));
+}
+
 // ---------------------------------------------------------------------------- select
 // One workgroup per (row, kv head).  The bound of a page is one dot product of
-// its two bound rows with the group's summed positive and negative parts of q;
+// its two bound rows with the group's summed positive and negative parts of q, in
 // fp64, so that the order is the formula's and not the summation's (products of a
-// 24-bit q and a 4-bit code are exact).  The top_k-th score is then found by its
-// bits, and the chosen pages written in ascending order.
-constexpr int SEL_THREADS = 256;
+// 24-bit q and a 4-bit code are exact).  D / 8 lanes read a page, four pages at a
+// time: their sums fold into each other, half the lanes keeping half the pages at
+// each step.  The smallest taken key is then found by its digits, from the highest
+// bit in which keys differ, and the chosen pages are written in ascending order.
+// Bound by latency (page ids, then bounds) and by the conversions to fp64.
 constexpr int SEL_MAX_WIDTH = 16384;        // scores of a row in LDS
 
 // order-preserving map of a score: NaN as +inf, an absent page 0
@@ -306,151 +438,210 @@ __device__ __forceinline__ uint64_t score_key64(double s) {
     return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(SEL_THREADS)
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(NT)
 select_pages_kernel(ssa_select_pages_args a) {
+    constexpr int LP = D / 8, NW = NT / SSA_WAVE, PARTS = NT / D;   // LP lanes of 16 codes a page
     extern __shared__ uint64_t sel_keys[];
-    __shared__ double qsum[2 * D];
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t digit, left_s;
-    __shared__ int wave_cnt[SEL_THREADS / SSA_WAVE];
+    __shared__ double qsum[PARTS * 2 * D];
+    __shared__ uint32_t hist[2][256];
+    __shared__ uint32_t digit, left_s, max_hi, min_hi;
+    __shared__ int gt_cnt[NW], eq_cnt[NW];
     const ssa_kv_cache &c = a.cache;
     const int t = (int)blockIdx.x, h = (int)blockIdx.y, tid = (int)threadIdx.x;
+    const int lane = lane_id(), wave = tid / SSA_WAVE;
     const int rep = a.Hq / c.Hkv;
     int32_t *out = a.out + ((int64_t)t * c.Hkv + h) * a.top_k;
     const int r = a.rows.requests[t], pos = a.rows.positions[t];
     int n = 0;
     if (r >= 0 && r < a.rows.R && pos >= 0) n = min(pos / c.page + 1, a.rows.width);
     if (n <= a.top_k) {
-        for (int i = tid; i < a.top_k; i += SEL_THREADS) out[i] = i < n ? i : -1;
+        for (int i = tid; i < a.top_k; i += NT) out[i] = i < n ? i : -1;
         return;
     }
-    // group's sums of the positive parts (for hi) and the negative ones (for lo)
-    for (int x = tid; x < D; x += SEL_THREADS) {
+    // the group's sums of the negative parts of q (for the smallest key codes) and
+    // of the positive ones (for the largest)
+    {
+        const int x = tid % D, part = tid / D;
         double p = 0., m = 0.;
         if (x < c.d)
-            for (int g = 0; g < rep; ++g) {
-                const float v = to_f32(((const T *)a.q)[t * a.q_st + (int64_t)(h * rep + g) * a.q_sh + x]);
-                if (v != v) p = m = (double)v;              // NaN stays
-                else if (v > 0.f) p += (double)v;
-                else m += (double)v;
+            for (int g = part; g < rep; g += PARTS) {
+                const float v =
+                    to_f32(((const T *)a.q)[t * a.q_st + (int64_t)(h * rep + g) * a.q_sh + x]);
+                p += (double)(v < 0.f ? 0.f : v);           // a NaN stays in both
+                m += (double)(v > 0.f ? 0.f : v);
             }
-        qsum[x] = m;
-        qsum[D + x] = p;
+        qsum[part * 2 * D + x] = m;
+        qsum[part * 2 * D + D + x] = p;
+    }
+    if (tid < 256) hist[0][tid] = 0;
+    if (tid == 0) {
+        max_hi = 0;
+        min_hi = ~0u;
     }
     __syncthreads();
-    const int first = min(a.first, n), last = max(n - a.recent, first);
-    constexpr int LP = D / 8;                               // lanes of a page: 16 codes each
     const int sub = tid % LP;
     double qr[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) qr[j] = qsum[sub * 16 + j];
+    for (int j = 0; j < 16; ++j) {
+        qr[j] = qsum[sub * 16 + j];
+#pragma unroll
+        for (int i = 1; i < PARTS; ++i) qr[j] += qsum[i * 2 * D + sub * 16 + j];
+    }
+    const int first = min(a.first, n), last = max(n - a.recent, first);
     const int32_t *table = a.rows.block_table + (int64_t)r * a.rows.table_stride;
-    for (int p = first + tid / LP; p < last; p += SEL_THREADS / LP) {
-        const int pg = table[p];
-        const bool there = pg >= 0 && pg < c.num_pages;
-        double s = 0.;
-        if (there) {
-            const int64_t ph = (int64_t)pg * c.Hkv + h;
-            const uint4 w = ((const uint4 *)((const uint8_t *)c.bounds + ph * 2 * D))[sub];
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    uint32_t mx = 0, mn = ~0u;
+    for (int p0 = first + tid / LP * 4; p0 < last; p0 += NT / LP * 4) {
+        int pg[4];
+        uint4 w[4];
+        float sc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pg[i] = p0 + i < last ? table[p0 + i] : -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t ph = (int64_t)(pg[i] >= 0 && pg[i] < c.num_pages ? pg[i] : 0) * c.Hkv + h;
+            w[i] = ((const uint4 *)((const uint8_t *)c.bounds + ph * 2 * D))[sub];
+            sc[i] = c.k_scale[ph];
+        }
+        double s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            s[i] = 0.;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                s = fma((double)code_f32<0>(ws[j]), qr[4 * j], s);
-                s = fma((double)code_f32<1>(ws[j]), qr[4 * j + 1], s);
-                s = fma((double)code_f32<2>(ws[j]), qr[4 * j + 2], s);
-                s = fma((double)code_f32<3>(ws[j]), qr[4 * j + 3], s);
+                s[i] = fma((double)code_f32<0>(ws[j]), qr[4 * j], s[i]);
+                s[i] = fma((double)code_f32<1>(ws[j]), qr[4 * j + 1], s[i]);
+                s[i] = fma((double)code_f32<2>(ws[j]), qr[4 * j + 2], s[i]);
+                s[i] = fma((double)code_f32<3>(ws[j]), qr[4 * j + 3], s[i]);
             }
-            s *= (double)c.k_scale[ph];
+            s[i] *= (double)sc[i];
         }
+        // lanes of the upper half keep pages 2 and 3, then of each quarter one page;
+        // every page's sum is the same tree over its lanes
+        const bool ua = sub & (LP / 2), ub = sub & (LP / 4);
+        double k0 = ua ? s[2] : s[0], k1 = ua ? s[3] : s[1];
+        k0 += __shfl_xor(ua ? s[0] : s[2], LP / 2, SSA_WAVE);
+        k1 += __shfl_xor(ua ? s[1] : s[3], LP / 2, SSA_WAVE);
+        double v = ub ? k1 : k0;
+        v += __shfl_xor(ub ? k0 : k1, LP / 4, SSA_WAVE);
 #pragma unroll
-        for (int o = LP / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, SSA_WAVE);
-        if (sub == 0) sel_keys[p - first] = there ? score_key64(s) : 0;
+        for (int o = LP / 8; o > 0; o >>= 1) v += __shfl_xor(v, o, SSA_WAVE);
+        const int i = (ua ? 2 : 0) + (ub ? 1 : 0), p = p0 + i;
+        if (sub % (LP / 4) == 0 && p < last) {
+            const int pi = i == 0 ? pg[0] : (i == 1 ? pg[1] : (i == 2 ? pg[2] : pg[3]));
+            const uint64_t key = pi >= 0 && pi < c.num_pages ? score_key64(v) : 0;
+            sel_keys[p - first] = key;
+            mx = max(mx, (uint32_t)(key >> 32));
+            mn = min(mn, (uint32_t)(key >> 32));
+        }
+    }
+    mx = wave_max_u(mx);
+    mn = wave_min_u(mn);
+    if (lane == 0) {
+        atomicMax(&max_hi, mx);
+        atomicMin(&min_hi, mn);
     }
     __syncthreads();
-    // the need-th largest key among nc, and how many equal to it are taken
+    // the left-th largest of nc keys, digit by digit; the keys agree above the first
     const int nc = last - first;
     uint32_t left = (uint32_t)(a.top_k - first - (n - last));
-    uint64_t prefix = 0;
-    int shift = 56;
+    const uint32_t differ = max_hi ^ min_hi;
+    int shift = differ ? max(32 + 31 - __clz((int)differ) - 7, 0) : 24;
+    // keys >> (shift + 8) are the same for all at first
+    uint64_t prefix = ((uint64_t)max_hi << 32) >> shift >> 8;
+    int buf = 0, bits = 8;
     if (left > 0)
-    for (;; shift -= 8) {
-        hist[tid] = 0;
-        __syncthreads();
-        for (int i = tid; i < nc; i += SEL_THREADS) {
-            const uint64_t k = sel_keys[i];
-            if (shift == 56 || (k >> (shift + 8)) == prefix)
-                atomicAdd(&hist[(k >> shift) & 255], 1u);
+        for (;;) {
+            for (int i = tid; i < nc; i += NT) {
+                const uint64_t k = sel_keys[i] >> shift;
+                if ((k >> bits) == prefix)
+                    atomicAdd(&hist[buf][(uint32_t)k & ((1u << bits) - 1u)], 1u);
+            }
+            if (tid < 256) hist[buf ^ 1][tid] = 0;
+            __syncthreads();
+            if (wave == 0) {                // four digits a lane, sums from the top
+                uint32_t b[4], own = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) own += b[j] = hist[buf][4 * lane + j];
+                uint32_t suf = own;
+#pragma unroll
+                for (int o = 1; o < SSA_WAVE; o <<= 1) {
+                    const uint32_t u = (uint32_t)__shfl_down((int)suf, o, SSA_WAVE);
+                    if (lane + o < SSA_WAVE) suf += u;
+                }
+                uint32_t above = suf - own;
+#pragma unroll
+                for (int j = 3; j >= 0; --j) {
+                    if (above < left && above + b[j] >= left) {
+                        digit = (uint32_t)(4 * lane + j);
+                        left_s = left - above;
+                    }
+                    above += b[j];
+                }
+            }
+            __syncthreads();
+            left = left_s;
+            prefix = (prefix << bits) | digit;
+            if (shift == 0 || hist[buf][digit] == left) break;
+            bits = min(shift, 8);
+            shift -= bits;
+            buf ^= 1;
+            __syncthreads();                // digit and left are read
         }
-        __syncthreads();
-        // digit: the largest v with sum of hist[v..] >= left
-        uint32_t above = 0;
-        for (int v = tid + 1; v < 256; ++v) above += hist[v];
-        if (above < left && above + hist[tid] >= left) {
-            digit = (uint32_t)tid;
-            left_s = left - above;
-        }
-        __syncthreads();
-        left = left_s;
-        prefix = (prefix << 8) | digit;
-        const bool done = shift == 0 || hist[digit] == left;
-        __syncthreads();
-        if (done) break;
-    }
-    // pages above the prefix are taken, and the first `left` equal to it
-    int out_n = 0;
-    uint32_t eq_n = 0;
-    for (int b = 0; b < n; b += SEL_THREADS) {
+    // taken: the forced pages, those above the prefix, the first `left` equal to it
+    int gt0 = 0, eq0 = 0;
+    for (int b = 0; b < n; b += NT) {
         const int p = b + tid;
-        bool take = p < n && (p < first || p >= last), eq = false;
+        bool gt = p < n && (p < first || p >= last), eq = false;
         if (p >= first && p < last && left > 0) {
             const uint64_t k = sel_keys[p - first] >> shift;
-            take = k > prefix;
+            gt = k > prefix;
             eq = k == prefix;
         }
-        // ranks by two scans: of the equal ones, then of those taken
-        const int wave = tid / SSA_WAVE;
-        uint64_t m = wave_ballot(eq);
-        if (lane_id() == 0) wave_cnt[wave] = __popcll(m);
-        __syncthreads();
-        uint32_t er = eq_n + (uint32_t)lanes_below(m), ea = 0;
-        for (int w = 0; w < SEL_THREADS / SSA_WAVE; ++w) {
-            if (w < wave) er += (uint32_t)wave_cnt[w];
-            ea += (uint32_t)wave_cnt[w];
+        const uint64_t mg = wave_ballot(gt), me = wave_ballot(eq);
+        if (lane == 0) {
+            gt_cnt[wave] = __popcll(mg);
+            eq_cnt[wave] = __popcll(me);
         }
-        eq_n += ea;
-        take = take || (eq && er < left);
         __syncthreads();
-        m = wave_ballot(take);
-        if (lane_id() == 0) wave_cnt[wave] = __popcll(m);
-        __syncthreads();
-        int at = out_n + lanes_below(m), all = 0;
-        for (int w = 0; w < SEL_THREADS / SSA_WAVE; ++w) {
-            if (w < wave) at += wave_cnt[w];
-            all += wave_cnt[w];
+        int g = gt0 + lanes_below(mg), e = eq0 + lanes_below(me);
+        for (int w = 0; w < NW; ++w) {
+            if (w < wave) {
+                g += gt_cnt[w];
+                e += eq_cnt[w];
+            }
+            gt0 += gt_cnt[w];
+            eq0 += eq_cnt[w];
         }
-        out_n += all;
-        if (take && at < a.top_k) out[at] = p;
+        const int at = g + min(e, (int)left);
+        if ((gt || (eq && e < (int)left)) && at < a.top_k) out[at] = p;
         __syncthreads();
     }
-    for (int i = out_n + tid; i < a.top_k; i += SEL_THREADS) out[i] = -1;
 }
 
-template <typename T>
-void launch_select(const ssa_select_pages_args &a, hipStream_t s) {
-    const dim3 grid((unsigned)a.rows.T, (unsigned)a.cache.Hkv);
+template <typename T, int D, int NT>
+int launch_select(const ssa_select_pages_args &a, hipStream_t s) {
     const size_t lds = (size_t)a.rows.width * 8;
-    if (a.cache.D == 64) select_pages_kernel<T, 64><<<grid, SEL_THREADS, lds, s>>>(a);
-    else if (a.cache.D == 128) select_pages_kernel<T, 128><<<grid, SEL_THREADS, lds, s>>>(a);
-    else select_pages_kernel<T, 256><<<grid, SEL_THREADS, lds, s>>>(a);
+    SSA_ALLOW_LDS((select_pages_kernel<T, D, NT>), lds);
+    const dim3 grid((unsigned)a.rows.T, (unsigned)a.cache.Hkv);
+    select_pages_kernel<T, D, NT><<<grid, NT, lds, s>>>(a);
+    return SSA_OK;
+}
+
+// Few rows: a CU has one workgroup or none, and 16 waves shorten its walk over the
+// pages.  Many: 4 waves, so that several workgroups hide each other's latency.
+template <typename T, int D>
+int launch_select_d(const ssa_select_pages_args &a, hipStream_t s) {
+    return (int64_t)a.rows.T * a.cache.Hkv <= 512 ? launch_select<T, D, 1024>(a, s)
+                                                  : launch_select<T, D, 256>(a, s);
 }
 
 template <typename T>
-int allow_select_lds(size_t lds) {
-    SSA_ALLOW_LDS((select_pages_kernel<T, 64>), lds);
-    SSA_ALLOW_LDS((select_pages_kernel<T, 128>), lds);
-    SSA_ALLOW_LDS((select_pages_kernel<T, 256>), lds);
-    return SSA_OK;
+int launch_select_t(const ssa_select_pages_args &a, hipStream_t s) {
+    return a.cache.D == 64 ? launch_select_d<T, 64>(a, s)
+                           : (a.cache.D == 128 ? launch_select_d<T, 128>(a, s)
+                                               : launch_select_d<T, 256>(a, s));
 }
 
 }  // namespace
@@ -495,22 +686,11 @@ extern "C" int ssa_cache_append(const ssa_cache_append_args *a, void *stream) {
     SSA_CHECK_ARG(a->T >= 0, "cache_append: T=%d", a->T);
     if (a->T == 0) return SSA_OK;
     SSA_CHECK_ARG(a->k && a->v && a->slots, "cache_append: null pointer");
-    // a workgroup looks at `window` rows for the first rows of runs: one each while
-    // they all may be (single tokens), more where most lie inside a run
-    const int window = a->T <= 1024 ? 1 : (a->T <= 4096 ? 4 : 16);
-    const dim3 grid((unsigned)ceil_div(a->T, window), (unsigned)a->cache.Hkv);
-    const size_t lds = (size_t)2 * a->cache.page * a->cache.D;
     const hipStream_t s = (hipStream_t)stream;
-    if (a->dtype == SSA_F32) {
-        SSA_ALLOW_LDS(cache_append_kernel<float>, lds);
-        cache_append_kernel<float><<<grid, APP_THREADS, lds, s>>>(*a, window);
-    } else if (a->dtype == SSA_BF16) {
-        SSA_ALLOW_LDS(cache_append_kernel<bf16_t>, lds);
-        cache_append_kernel<bf16_t><<<grid, APP_THREADS, lds, s>>>(*a, window);
-    } else {
-        SSA_ALLOW_LDS(cache_append_kernel<f16_t>, lds);
-        cache_append_kernel<f16_t><<<grid, APP_THREADS, lds, s>>>(*a, window);
-    }
+    const int lc = a->dtype == SSA_F32 ? launch_append_t<float>(*a, s)
+                 : a->dtype == SSA_BF16 ? launch_append_t<bf16_t>(*a, s)
+                                        : launch_append_t<f16_t>(*a, s);
+    if (lc != SSA_OK) return lc;
     SSA_CHECK_LAUNCH();
     return SSA_OK;
 }
@@ -536,21 +716,11 @@ extern "C" int ssa_select_pages(const ssa_select_pages_args *a, void *stream) {
     }
     if (a->rows.T == 0) return SSA_OK;
     SSA_CHECK_ARG(a->q && a->out, "select_pages: null pointer");
-    const size_t lds = (size_t)a->rows.width * 8;
     const hipStream_t s = (hipStream_t)stream;
-    if (a->dtype == SSA_F32) {
-        rc = allow_select_lds<float>(lds);
-        if (rc != SSA_OK) return rc;
-        launch_select<float>(*a, s);
-    } else if (a->dtype == SSA_BF16) {
-        rc = allow_select_lds<bf16_t>(lds);
-        if (rc != SSA_OK) return rc;
-        launch_select<bf16_t>(*a, s);
-    } else {
-        rc = allow_select_lds<f16_t>(lds);
-        if (rc != SSA_OK) return rc;
-        launch_select<f16_t>(*a, s);
-    }
+    rc = a->dtype == SSA_F32 ? launch_select_t<float>(*a, s)
+       : a->dtype == SSA_BF16 ? launch_select_t<bf16_t>(*a, s)
+                              : launch_select_t<f16_t>(*a, s);
+    if (rc != SSA_OK) return rc;
     SSA_CHECK_LAUNCH();
     return SSA_OK;
 }
