@@ -13,207 +13,158 @@
 // (or 8) bytes, a wave 1 KB in one piece.  Key rows are read in 64-byte pieces.
 // Nothing passes through LDS but the waves' results.
 //
-// Codes become bf16 with their scale in one instruction for two
-// (v_cvt_scalef32_pk_bf16_fp8), exactly: a code has 4 significant bits and the
-// scale is a power of two.  q and p are split into bf16 terms whose sum has the
-// precision that is wanted (bf16 q 1 term, fp16 2, fp32 3; p 2 or 3), so every
-// product is exact and only fp32 sums round.
+// Codes become 16-bit floats in one instruction for two, exactly (a code has 4
+// significant bits), and queries are exact too, so products are and only fp32 sums
+// round; probabilities round to 11 bits, for fp32 queries to 24.
 #include "ssa_cache_attend_dev.h"
 
 namespace {
 
-// A workgroup takes 16 RT columns (query rows of one request and kv head) and a
-// chunk of the key tiles; its waves take every fourth tile of the chunk.
-template <typename T, int D, int KT, int RT>
-__global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE)
+// A unit is 16 RT columns.  SHARED: a workgroup takes one unit and a chunk of its key
+// tiles, its waves every fourth tile, and their sums are joined in LDS.  Otherwise
+// each wave takes a unit of its own and all of its tiles: no joining, for calls with
+// units enough to fill the chip.  A wave holds one tile's values and the next one's
+// keys in flight, and looks page ids up a tile ahead of those.
+template <typename T, int D, int KT, int RT, bool SHARED>
+__global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE, D <= 128 && RT == 1 ? 2 : 1)
 cache_attend_kernel(AttendParams p) {
-    constexpr int NQ = sizeof(T) == 4 ? 3 : (__is_same(T, f16_t) ? 2 : 1);
-    constexpr int NP = sizeof(T) == 4 ? 3 : 2;
-    constexpr int CT = 16 * RT, NB = KT / 16, DP = D / 64, ND = D / 16, KS = KT / 32;
-    constexpr int OS = D + 4;                 // row stride of the waves' sums in LDS
-    __shared__ float o_lds[CT * OS];
+    typedef Columns<T, D, KT, RT> C;
+    typedef typename C::PV PV;
+    constexpr int NQ = C::NQ, NP = C::NP, NB = C::NB, DP = C::DP, ND = C::ND, KS = C::KS;
+    constexpr int CT = 16 * RT, OS = D + 4;   // OS: row stride of the joined sums
+    __shared__ float o_lds[SHARED ? CT * OS : 1];
     __shared__ float m_lds[ATT_WAVES][CT], l_lds[ATT_WAVES][CT];
 
     const int lane = lane_id(), col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / SSA_WAVE);
-    const int h = (int)blockIdx.y, split = (int)blockIdx.z;
-
+    // kv heads run fastest: an XCD's workgroups share their heads' pages in its L2
+    const int h = (int)(blockIdx.x % (unsigned)p.Hkv), split = (int)blockIdx.y;
+    int u = (int)(blockIdx.x / (unsigned)p.Hkv);
+    if (!SHARED) u = u * ATT_WAVES + wave;
     Unit un;
-    if (!locate_unit(p, (int)blockIdx.x, CT, un)) return;
-    const int req = un.req, t0 = un.t0, c0 = un.c0, c1 = un.c1;
+    if (u >= p.units || !locate_unit(p, u, CT, un)) return;
+    C w;
+    w.start(p, un, un.c0, un.c1, h);
 
-    int pos[RT];                              // last key each column sees
-    int64_t qrow[RT];
-    int most = -1;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int c = c0 + rt * 16 + col;
-        const bool live = c < c1;
-        const int t = t0 + c / p.rep;
-        pos[rt] = live && req >= 0 && p.requests[t] == req ? p.positions[t] : -1;
-        qrow[rt] = live ? t * p.q_st + (int64_t)(h * p.rep + c % p.rep) * p.q_sh : -1;
-        most = max(most, pos[rt]);
-    }
-    most = __builtin_amdgcn_readfirstlane((int)wave_max_u((uint32_t)(most + 1))) - 1;
-    const int page = 1 << p.page_shift;
-    most = min(most, p.width * page - 1);
-
-    const int sub_tiles = page / KT;          // 1, or 2 for pages of 128
-    const int32_t *list = nullptr;
-    int n_tiles = most < 0 ? 0 : most / KT + 1;
-    if (p.pages) {
-        list = p.pages + ((int64_t)t0 * p.Hkv + h) * p.top;
-        n_tiles = most < 0 ? 0 : p.top * sub_tiles;
-    }
+    const int page = 1 << p.page_shift, sub_shift = p.page_shift - (KT == 64 ? 6 : 5);
+    const int32_t *list = p.pages ? p.pages + ((int64_t)un.t0 * p.Hkv + h) * p.top : nullptr;
+    const int32_t *table = p.table + (int64_t)(un.req < 0 ? 0 : un.req) * p.table_stride;
+    const int n_tiles = w.most < 0 ? 0 : (list ? p.top << sub_shift : w.most / KT + 1);
     const int tile0 = split * p.chunk, tile1 = min(tile0 + p.chunk, n_tiles);
+    constexpr int STEP = SHARED ? ATT_WAVES : 1;
 
-    bf16x8 qf[RT][DP * 2][NQ];
-    f32x4 o[RT][ND];
-    float m[RT], l[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -INFINITY;
-        l[rt] = 0.f;
-#pragma unroll
-        for (int i = 0; i < ND; ++i) o[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < DP * 2; ++s)
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) qf[rt][s][n] = bf16x8{};
-    }
-    if (tile0 < tile1) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int s = 0; s < DP * 2; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int x = (s >> 1) * 64 + g * 16 + (s & 1) * 8 + j;
-                    float v = qrow[rt] >= 0 && x < p.d ? to_f32(((const T *)p.q)[qrow[rt] + x]) : 0.f;
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) {
-                        const __bf16 b = (__bf16)v;
-                        qf[rt][s][n][j] = b;
-                        v -= (float)b;
-                    }
-                }
-    }
-
-    const int32_t *table = p.table + (int64_t)(req < 0 ? 0 : req) * p.table_stride;
-    for (int tile = tile0 + wave; tile < tile1; tile += ATT_WAVES) {
-        int lp = tile / sub_tiles;
-        const int sub = tile - lp * sub_tiles;
-        if (list) lp = list[lp];
-        if (lp < 0 || lp >= p.width) continue;
+    // logical page of a tile; its place in the cache, -1 if it is absent or unseen
+    auto logical = [&](int tile) {
+        if (tile >= tile1) return -1;
+        return list ? list[tile >> sub_shift] : tile >> sub_shift;
+    };
+    auto place = [&](int tile, int lp) {
+        if (lp < 0 || lp >= p.width || (lp << p.page_shift) + (tile & ((1 << sub_shift) - 1)) * KT > w.most)
+            return -1;
         const int pg = table[lp];
-        if (pg < 0 || pg >= p.num_pages) continue;
-        const int key0 = lp * page + sub * KT;
-        if (key0 > most) continue;
+        return pg >= 0 && pg < p.num_pages ? pg : -1;
+    };
+    uint4 kr[NB][DP];
+    float ks = 0.f, vs = 0.f;
+    auto fetch_keys = [&](int tile, int pg) {
+        if (pg < 0) return;
         const int64_t ph = (int64_t)pg * p.Hkv + h;
-        const float ks = p.ks[ph], vs = p.vs[ph];
-        const uint8_t *kb = p.k + ph * page * D + (int64_t)sub * KT * D;
-        const uint8_t *vb = p.v + ph * D * page + sub * KT;
+        ks = p.ks[ph];
+        vs = p.vs[ph];
+        const uint8_t *kb = p.k + ph * page * D + (int64_t)(tile & ((1 << sub_shift) - 1)) * KT * D;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < DP; ++i)
+                kr[b][i] = *(const uint4 *)(kb + (KT / 4 * (col >> 2) + 4 * b + (col & 3)) * D + i * 64 + g * 16);
+    };
 
-        f32x4 s[RT][NB];
+    int tile = tile0 + (SHARED ? wave : 0);
+    int lp = logical(tile), pg = place(tile, lp), lp1 = logical(tile + STEP);
+    fetch_keys(tile, pg);
+    for (; tile < tile1; tile += STEP) {
+        const int pg1 = place(tile + STEP, lp1), lp2 = logical(tile + 2 * STEP);
+        if (pg >= 0) {
+            const int sub = tile & ((1 << sub_shift) - 1);
+            const float kscale = ks, vscale = vs;
+            const uint8_t *vb = p.v + ((int64_t)pg * p.Hkv + h) * D * page + sub * KT;
+            uint32_t vr[ND][KT / 16];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int key = KT / 4 * (col >> 2) + 4 * b + (col & 3);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < DP; ++i) {
-                const uint4 w = *(const uint4 *)(kb + key * D + i * 64 + g * 16);
-                const bf16x8 k0 = codes_bf16(w.x, w.y, ks), k1 = codes_bf16(w.z, w.w, ks);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int n = NQ - 1; n >= 0; --n) {
-                        s[rt][b] = mfma(k0, qf[rt][2 * i][n], s[rt][b]);
-                        s[rt][b] = mfma(k1, qf[rt][2 * i + 1][n], s[rt][b]);
-                    }
+            for (int i = 0; i < ND; ++i) {
+                const uint8_t *at = vb + ((i * 16 + col) << p.page_shift) + KT / 4 * g;
+                if constexpr (KT == 64) {
+                    const uint4 x = *(const uint4 *)at;
+                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][2] = x.z; vr[i][3] = x.w;
+                } else {
+                    const uint2 x = *(const uint2 *)at;
+                    vr[i][0] = x.x; vr[i][1] = x.y;
+                }
             }
+            f32x4 s[RT][NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) s[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < DP; ++i) {
+                    const uint4 x = kr[b][i];
+                    const typename C::QV k0 = Ops<T>::key(x.x, x.y), k1 = Ops<T>::key(x.z, x.w);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int n = NQ - 1; n >= 0; --n) {
+                            s[rt][b] = mfma(k0, w.q[rt][2 * i][n], s[rt][b]);
+                            s[rt][b] = mfma(k1, w.q[rt][2 * i + 1][n], s[rt][b]);
+                        }
+                }
+            }
+            fetch_keys(tile + STEP, pg1);
+            PV pf[RT][KS][NP];
+            w.softmax(s, kscale, vscale, (lp << p.page_shift) + sub * KT, pf);
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    const PV vf = Ops<T>::value(vr[i][2 * k], vr[i][2 * k + 1], vscale);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int n = NP - 1; n >= 0; --n)
+                            w.o[rt][i] = mfma(vf, pf[rt][k][n], w.o[rt][i]);
+                }
+        } else {
+            fetch_keys(tile + STEP, pg1);
         }
-        bf16x8 pf[RT][KS][NP];
+        lp = lp1;
+        pg = pg1;
+        lp1 = lp2;
+    }
+    if constexpr (!SHARED) {
+        w.finish(p, un, un.c0, un.c1, h, split, tile0 < tile1);
+        return;
+    }
+
+    // join the waves: m, l, O in the waves' order
+    if (g == 0)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float mx = m[rt];
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int key = key0 + KT / 4 * g + 4 * b + r;
-                    const float v = key <= pos[rt] ? s[rt][b][r] * p.scale : -INFINITY;
-                    s[rt][b][r] = v;
-                    mx = fmaxf(mx, v);
-                }
-            mx = fmaxf(mx, __shfl_xor(mx, 16, SSA_WAVE));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, SSA_WAVE));
-            const float ms = mx == -INFINITY ? 0.f : mx;
-            const float a = __builtin_amdgcn_exp2f(m[rt] - ms);
-            m[rt] = mx;
-            float sum = 0.f;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float v = __builtin_amdgcn_exp2f(s[rt][b][r] - ms);
-                    sum += v;
-#pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        const __bf16 t = (__bf16)v;
-                        pf[rt][b >> 1][n][(b & 1) * 4 + r] = t;
-                        v -= (float)t;
-                    }
-                }
-            l[rt] = l[rt] * a + sum;
-#pragma unroll
-            for (int i = 0; i < ND; ++i) o[rt][i] *= a;
+            m_lds[wave][rt * 16 + col] = w.m[rt];
+            l_lds[wave][rt * 16 + col] = w.l[rt][0];
         }
-#pragma unroll
-        for (int i = 0; i < ND; ++i) {
-            const uint8_t *at = vb + (int64_t)(i * 16 + col) * page + KT / 4 * g;
-            uint32_t w[KT / 16];
-            if constexpr (KT == 64) {
-                const uint4 u = *(const uint4 *)at;
-                w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-            } else {
-                const uint2 u = *(const uint2 *)at;
-                w[0] = u.x; w[1] = u.y;
-            }
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const bf16x8 vf = codes_bf16(w[2 * k], w[2 * k + 1], vs);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int n = NP - 1; n >= 0; --n) o[rt][i] = mfma(vf, pf[rt][k][n], o[rt][i]);
-            }
-        }
-    }
-
-    // join the waves: l over the lane groups, then m, l, O over the waves in order
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        l[rt] += __shfl_xor(l[rt], 16, SSA_WAVE);
-        l[rt] += __shfl_xor(l[rt], 32, SSA_WAVE);
-        if (g == 0) {
-            m_lds[wave][rt * 16 + col] = m[rt];
-            l_lds[wave][rt * 16 + col] = l[rt];
-        }
-    }
     __syncthreads();
-    for (int w = 0; w < ATT_WAVES; ++w) {
-        if (w == wave) {
+    const float unit = w.unit();
+    for (int v = 0; v < ATT_WAVES; ++v) {
+        if (v == wave) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 float mx = -INFINITY;
-                for (int v = 0; v < ATT_WAVES; ++v) mx = fmaxf(mx, m_lds[v][rt * 16 + col]);
-                const float a = __builtin_amdgcn_exp2f(m[rt] - (mx == -INFINITY ? 0.f : mx));
+                for (int i = 0; i < ATT_WAVES; ++i) mx = fmaxf(mx, m_lds[i][rt * 16 + col]);
+                const float a = __builtin_amdgcn_exp2f(w.m[rt] - (mx == -INFINITY ? 0.f : mx)) * unit;
 #pragma unroll
                 for (int i = 0; i < ND; ++i) {
                     f32x4 *at = (f32x4 *)&o_lds[(rt * 16 + col) * OS + i * 16 + 4 * g];
-                    const f32x4 x = o[rt][i] * a;
-                    *at = w == 0 ? x : *at + x;
+                    const f32x4 x = w.o[rt][i] * a;
+                    *at = v == 0 ? x : *at + x;
                 }
             }
         }
@@ -221,13 +172,13 @@ cache_attend_kernel(AttendParams p) {
     }
     for (int i = (int)threadIdx.x; i < CT * D; i += ATT_WAVES * SSA_WAVE) {
         const int c = i / D, x = i - c * D;
-        if (c0 + c >= c1) break;
+        if (un.c0 + c >= un.c1) break;
         float mx = -INFINITY, sum = 0.f;
         for (int v = 0; v < ATT_WAVES; ++v) mx = fmaxf(mx, m_lds[v][c]);
         const float ms = mx == -INFINITY ? 0.f : mx;
         for (int v = 0; v < ATT_WAVES; ++v)
             sum += l_lds[v][c] * __builtin_amdgcn_exp2f(m_lds[v][c] - ms);
-        const int t = t0 + (c0 + c) / p.rep, hq = h * p.rep + (c0 + c) % p.rep;
+        const int t = un.t0 + (un.c0 + c) / p.rep, hq = h * p.rep + (un.c0 + c) % p.rep;
         const float v = o_lds[c * OS + x];
         if (p.S == 1) {
             if (x < p.d)
@@ -249,12 +200,22 @@ cache_attend_kernel(AttendParams p) {
 template <typename T, int D>
 __global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE)
 cache_join_kernel(AttendParams p, int CT) {
-    Unit un;
-    if (!locate_unit(p, (int)blockIdx.x, CT, un)) return;
-    const int c = un.c0 + (int)blockIdx.z * ATT_WAVES + (int)threadIdx.x / SSA_WAVE;
-    if (c >= un.c1) return;
     const int lane = lane_id();
-    const int t = un.t0 + c / p.rep, hq = (int)blockIdx.y * p.rep + c % p.rep;
+    const int i = (int)blockIdx.x * ATT_WAVES + (int)threadIdx.x / SSA_WAVE;
+    int t, hq;
+    if (p.mode == UNITS_PAGES || p.mode == UNITS_ALL) {    // every row
+        if (i >= p.T * p.Hq) return;
+        t = i / p.Hq;
+        hq = i - t * p.Hq;
+    } else {
+        Unit un;
+        const int u = i / CT;
+        if (u >= p.units || !locate_unit(p, u, CT, un)) return;
+        const int c = un.c0 + i - u * CT;
+        if (c >= un.c1) return;
+        t = un.t0 + c / p.rep;
+        hq = (int)blockIdx.y * p.rep + c % p.rep;
+    }
     const int64_t row = ((int64_t)t * p.Hq + hq) * p.s_stride;
     float mx = -INFINITY;
     for (int s = lane; s < p.S; s += SSA_WAVE) mx = fmaxf(mx, p.part_ml[2 * (row + s)]);
@@ -304,8 +265,8 @@ struct AttendShape {
     int RT, KT, S, chunk;                     // of the kernel above
     int mode;
     int64_t units;
-    bool prompt;
-    int prompt_S, prompt_chunk, prompt_cols;
+    bool shared, prompt;
+    int prompt_S, prompt_chunk, prompt_RT;
     int64_t prompt_units;
     int s_stride;
 };
@@ -326,7 +287,9 @@ AttendShape attend_shape(const ssa_cached_attention_args *a) {
     const int64_t T = a->rows.T, R = a->rows.R;
     const int rep = a->Hq / c.Hkv;
     s.KT = c.page < 64 ? 32 : 64;
-    s.RT = rep > 16 ? 2 : 1;
+    // two tiles of heads share a wave's keys where the registers hold both
+    s.RT = rep > 16 && c.D <= 128 ? 2 : 1;
+    s.shared = true;
     const int CT = 16 * s.RT;
     const int per_page = c.page / s.KT;
     int64_t tiles = (int64_t)a->rows.width * per_page;   // the most that a unit can have
@@ -341,12 +304,21 @@ AttendShape attend_shape(const ssa_cached_attention_args *a) {
         s.mode = UNITS_FEW;
         s.units = (R + 1) * ceil_div(MANY, CT);
         s.prompt = true;
-        s.prompt_cols = ssa_cache_prompt_columns(a->dtype, c.D);
-        s.prompt_units = T * rep / s.prompt_cols + R + 1;
-        split_tiles(tiles, s.prompt_units * c.Hkv, 512, 16, &s.prompt_S, &s.prompt_chunk);
+        // columns per wave: as many as leave two workgroups for every CU
+        s.prompt_RT = ssa_cache_prompt_max_rt(a->dtype, c.D);
+        for (;; s.prompt_RT /= 2) {
+            s.prompt_units = T * rep / (ATT_WAVES * 16 * s.prompt_RT) + R + 1;
+            if (s.prompt_RT == 1 || s.prompt_units * c.Hkv >= 512) break;
+        }
+        split_tiles(tiles, s.prompt_units * c.Hkv, 512, 4, &s.prompt_S, &s.prompt_chunk);
     }
     // two tiles or more for each wave
     split_tiles(tiles, s.units * c.Hkv, 2048, 2 * ATT_WAVES, &s.S, &s.chunk);
+    if (!s.prompt && s.units * c.Hkv >= 4096) {
+        s.shared = false;
+        s.S = 1;
+        s.chunk = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
+    }
     s.s_stride = s.prompt && s.prompt_S > s.S ? s.prompt_S : s.S;
     return s;
 }
@@ -372,14 +344,21 @@ int check_attend(const ssa_cached_attention_args *a) {
 template <typename T, int D>
 void launch_join(AttendParams p, int CT, hipStream_t st) {
     if (p.S == 1) return;
-    const dim3 grid((unsigned)p.units, (unsigned)p.Hkv, (unsigned)ceil_div(CT, ATT_WAVES));
+    const bool all = p.mode == UNITS_PAGES || p.mode == UNITS_ALL;
+    const int64_t columns = all ? (int64_t)p.T * p.Hq : (int64_t)p.units * CT;
+    const dim3 grid((unsigned)ceil_div(columns, ATT_WAVES), all ? 1u : (unsigned)p.Hkv);
     cache_join_kernel<T, D><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p, CT);
 }
 
 template <typename T, int D, int KT, int RT>
 void launch_attend(const AttendParams &p, const AttendShape &s, hipStream_t st) {
-    const dim3 grid((unsigned)p.units, (unsigned)p.Hkv, (unsigned)p.S);
-    cache_attend_kernel<T, D, KT, RT><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
+    if (s.shared) {
+        const dim3 grid((unsigned)(p.units * p.Hkv), (unsigned)p.S);
+        cache_attend_kernel<T, D, KT, RT, true><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
+    } else {
+        const unsigned grid = (unsigned)(ceil_div(p.units, ATT_WAVES) * p.Hkv);
+        cache_attend_kernel<T, D, KT, RT, false><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
+    }
     launch_join<T, D>(p, 16 * RT, st);
     if (s.prompt) {
         AttendParams pp = p;
@@ -388,20 +367,21 @@ void launch_attend(const AttendParams &p, const AttendShape &s, hipStream_t st) 
         pp.S = s.prompt_S;
         pp.chunk = s.prompt_chunk;
         ssa_cache_prompt_launch(pp, sizeof(T) == 4 ? SSA_F32 : (__is_same(T, f16_t) ? SSA_F16 : SSA_BF16),
-                                D, KT, st);
-        launch_join<T, D>(pp, s.prompt_cols, st);
+                                D, KT, s.prompt_RT, st);
+        launch_join<T, D>(pp, ATT_WAVES * 16 * s.prompt_RT, st);
     }
 }
 
 template <typename T, int D>
 void launch_attend_d(const AttendParams &p, const AttendShape &s, hipStream_t st) {
-    if (s.KT == 32) {
-        if (s.RT == 1) launch_attend<T, D, 32, 1>(p, s, st);
-        else launch_attend<T, D, 32, 2>(p, s, st);
-    } else {
-        if (s.RT == 1) launch_attend<T, D, 64, 1>(p, s, st);
-        else launch_attend<T, D, 64, 2>(p, s, st);
-    }
+    if constexpr (D <= 128)
+        if (s.RT == 2) {
+            if (s.KT == 32) launch_attend<T, D, 32, 2>(p, s, st);
+            else launch_attend<T, D, 64, 2>(p, s, st);
+            return;
+        }
+    if (s.KT == 32) launch_attend<T, D, 32, 1>(p, s, st);
+    else launch_attend<T, D, 64, 1>(p, s, st);
 }
 
 template <typename T>
@@ -435,7 +415,7 @@ extern "C" int ssa_cached_attention(const ssa_cached_attention_args *a, void *wo
     }
     SSA_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "cached_attention: workspace alignment");
     const AttendShape s = attend_shape(a);
-    SSA_CHECK_ARG(s.units < (1ll << 31) && s.S <= 65535 &&
+    SSA_CHECK_ARG(s.units * a->cache.Hkv < (1ll << 31) && s.S <= 65535 &&
                       s.prompt_units * a->cache.Hkv < (1ll << 31) && s.prompt_S <= 65535,
                   "cached_attention: too many rows");
     const ssa_kv_cache &c = a->cache;
