@@ -11,7 +11,6 @@
 // stand for: in a tile of KT keys, row 4g + r of block b is key KT/4 g + 4b + r,
 // and lane group g then reads KT/4 adjacent tokens of a transposed value row: 16
 // (or 8) bytes, a wave 1 KB in one piece.  Key rows are read in 64-byte pieces.
-// Nothing passes through LDS but the waves' results.
 //
 // Codes become 16-bit floats in one instruction for two, exactly (a code has 4
 // significant bits), and queries are exact too, so products are and only fp32 sums
@@ -32,7 +31,10 @@ cache_attend_kernel(AttendParams p) {
     typedef typename C::PV PV;
     constexpr int NQ = C::NQ, NP = C::NP, NB = C::NB, DP = C::DP, ND = C::ND, KS = C::KS;
     constexpr int CT = 16 * RT, OS = D + 4;   // OS: row stride of the joined sums
-    __shared__ float o_lds[SHARED ? CT * OS : 1];
+    // each wave's pieces on their way to other lanes; then the joined sums
+    constexpr int XW = KT * D / 16, XN = ATT_WAVES * XW, ON = SHARED ? CT * OS / 4 : 0;
+    __shared__ u32x4 x_lds[XN > ON ? XN : ON];
+    float *o_lds = (float *)x_lds;
     __shared__ float m_lds[ATT_WAVES][CT], l_lds[ATT_WAVES][CT];
 
     const int lane = lane_id(), col = lane & 15, g = lane >> 4;
@@ -53,18 +55,22 @@ cache_attend_kernel(AttendParams p) {
     const int tile0 = split * p.chunk, tile1 = min(tile0 + p.chunk, n_tiles);
     constexpr int STEP = SHARED ? ATT_WAVES : 1;
 
-    // logical page of a tile; its place in the cache, -1 if it is absent or unseen
-    auto logical = [&](int tile) {
-        if (tile >= tile1) return -1;
-        return list ? list[tile >> sub_shift] : tile >> sub_shift;
+    // The logical page of a tile and its entry in the table, looked up a tile ahead
+    // of its keys: the loads are unconditional (of some entry that is there) and
+    // what they say is judged only where it is needed, so nothing waits for them.
+    const int last_entry = (max(tile1, 1) - 1) >> sub_shift;
+    auto look_up = [&](int tile) { return list ? list[min(tile >> sub_shift, last_entry)] : tile >> sub_shift; };
+    auto entry = [&](int lp) { return table[max(0, min(lp, p.width - 1))]; };
+    // the page's place in the cache, -1 if it is absent or unseen
+    auto place = [&](int tile, int lp, int pg) {
+        const int key0 = (lp << p.page_shift) + (tile & ((1 << sub_shift) - 1)) * KT;
+        return tile < tile1 && lp >= 0 && lp < p.width && key0 <= w.most && pg >= 0 && pg < p.num_pages
+                   ? pg : -1;
     };
-    auto place = [&](int tile, int lp) {
-        if (lp < 0 || lp >= p.width || (lp << p.page_shift) + (tile & ((1 << sub_shift) - 1)) * KT > w.most)
-            return -1;
-        const int pg = table[lp];
-        return pg >= 0 && pg < p.num_pages ? pg : -1;
-    };
-    uint4 kr[NB][DP];
+    u32x4 *xk = x_lds + wave * XW;            // [block][64 columns][slot]
+    u32x2 *xv = (u32x2 *)xk;                  // pages of 32: [16 columns][slot]
+    const int lrow = lane >> 2, lpiece = lane & 3, to = slot_of(lrow, lpiece), from = slot_of(col, g);
+    u32x4 kr[NB][DP];
     float ks = 0.f, vs = 0.f;
     auto fetch_keys = [&](int tile, int pg) {
         if (pg < 0) return;
@@ -76,14 +82,19 @@ cache_attend_kernel(AttendParams p) {
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int i = 0; i < DP; ++i)
-                kr[b][i] = *(const uint4 *)(kb + (KT / 4 * (col >> 2) + 4 * b + (col & 3)) * D + i * 64 + g * 16);
+                kr[b][i] = *(const u32x4 *)(kb + (KT / 4 * (lrow >> 2) + 4 * b + (lrow & 3)) * D + i * 64 + lpiece * 16);
     };
 
     int tile = tile0 + (SHARED ? wave : 0);
-    int lp = logical(tile), pg = place(tile, lp), lp1 = logical(tile + STEP);
-    fetch_keys(tile, pg);
+    int lp = 0, lp1 = 0, pg = -1;
+    if (tile < tile1) {
+        lp = look_up(tile);
+        lp1 = look_up(tile + STEP);
+        pg = place(tile, lp, entry(lp));
+        fetch_keys(tile, pg);
+    }
     for (; tile < tile1; tile += STEP) {
-        const int pg1 = place(tile + STEP, lp1), lp2 = logical(tile + 2 * STEP);
+        int pg1, lp2;
         if (pg >= 0) {
             const int sub = tile & ((1 << sub_shift) - 1);
             const float kscale = ks, vscale = vs;
@@ -91,15 +102,24 @@ cache_attend_kernel(AttendParams p) {
             uint32_t vr[ND][KT / 16];
 #pragma unroll
             for (int i = 0; i < ND; ++i) {
-                const uint8_t *at = vb + ((i * 16 + col) << p.page_shift) + KT / 4 * g;
+                const uint8_t *at = vb + ((i * 16 + lrow) << p.page_shift) + KT / 4 * lpiece;
                 if constexpr (KT == 64) {
-                    const uint4 x = *(const uint4 *)at;
+                    const u32x4 x = *(const u32x4 *)at;
                     vr[i][0] = x.x; vr[i][1] = x.y; vr[i][2] = x.z; vr[i][3] = x.w;
                 } else {
-                    const uint2 x = *(const uint2 *)at;
+                    const u32x2 x = *(const u32x2 *)at;
                     vr[i][0] = x.x; vr[i][1] = x.y;
                 }
             }
+            // loads go out in this order: values, then what the next tile's need
+            __builtin_amdgcn_sched_barrier(0);
+            const int entry1 = entry(lp1);
+            lp2 = look_up(tile + 2 * STEP);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < DP; ++i) xk[(b * DP + i) * SSA_WAVE + to] = kr[b][i];
+            wave_lds_sync();
             f32x4 s[RT][NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -107,7 +127,7 @@ cache_attend_kernel(AttendParams p) {
                 for (int rt = 0; rt < RT; ++rt) s[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < DP; ++i) {
-                    const uint4 x = kr[b][i];
+                    const u32x4 x = xk[(b * DP + i) * SSA_WAVE + from];
                     const typename C::QV k0 = Ops<T>::key(x.x, x.y), k1 = Ops<T>::key(x.z, x.w);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
@@ -118,11 +138,29 @@ cache_attend_kernel(AttendParams p) {
                         }
                 }
             }
+            pg1 = place(tile + STEP, lp1, entry1);
             fetch_keys(tile + STEP, pg1);
+            __builtin_amdgcn_sched_barrier(0);
             PV pf[RT][KS][NP];
             w.softmax(s, kscale, vscale, (lp << p.page_shift) + sub * KT, pf);
+            wave_lds_sync();
 #pragma unroll
-            for (int i = 0; i < ND; ++i)
+            for (int i = 0; i < ND; ++i) {
+                if constexpr (KT == 64)
+                    xk[i * SSA_WAVE + to] = u32x4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]};
+                else
+                    xv[i * SSA_WAVE + to] = u32x2{vr[i][0], vr[i][1]};
+            }
+            wave_lds_sync();
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                if constexpr (KT == 64) {
+                    const u32x4 x = xk[i * SSA_WAVE + from];
+                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][2] = x.z; vr[i][3] = x.w;
+                } else {
+                    const u32x2 x = xv[i * SSA_WAVE + from];
+                    vr[i][0] = x.x; vr[i][1] = x.y;
+                }
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
                     const PV vf = Ops<T>::value(vr[i][2 * k], vr[i][2 * k + 1], vscale);
@@ -132,7 +170,11 @@ cache_attend_kernel(AttendParams p) {
                         for (int n = NP - 1; n >= 0; --n)
                             w.o[rt][i] = mfma(vf, pf[rt][k][n], w.o[rt][i]);
                 }
+            }
+            wave_lds_sync();
         } else {
+            lp2 = look_up(tile + 2 * STEP);
+            pg1 = place(tile + STEP, lp1, entry(lp1));
             fetch_keys(tile + STEP, pg1);
         }
         lp = lp1;
@@ -151,7 +193,7 @@ cache_attend_kernel(AttendParams p) {
             m_lds[wave][rt * 16 + col] = w.m[rt];
             l_lds[wave][rt * 16 + col] = w.l[rt][0];
         }
-    __syncthreads();
+    __syncthreads();                          // (and no wave's pieces are read any more)
     const float unit = w.unit();
     for (int v = 0; v < ATT_WAVES; ++v) {
         if (v == wave) {
@@ -455,6 +497,10 @@ extern "C" int ssa_cached_attention(const ssa_cached_attention_args *a, void *wo
     p.units = (int32_t)s.units;
     p.chunk = s.chunk;
     p.scale = a->scale * LOG2E;
+    const int es = a->dtype == SSA_F32 ? 4 : 2;
+    p.q_vec = c.d % 8 == 0 && ((a->q_st | a->q_sh) * es) % 16 == 0 && ((uintptr_t)a->q & 15) == 0;
+    p.o_vec = c.d % 4 == 0 && ((a->o_st | a->o_sh) * es) % (4 * es) == 0 &&
+              ((uintptr_t)a->out & (4 * es - 1)) == 0;
     const hipStream_t st = (hipStream_t)stream;
     if (a->dtype == SSA_F32) launch_attend_t<float>(p, s, c.D, st);
     else if (a->dtype == SSA_BF16) launch_attend_t<bf16_t>(p, s, c.D, st);

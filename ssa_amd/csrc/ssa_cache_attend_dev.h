@@ -8,6 +8,8 @@ typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
 constexpr int ATT_WAVES = 4;                  // of a workgroup
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -30,6 +32,7 @@ struct AttendParams {
     float *part_ml, *part_o;                  // (T * Hq, s_stride, 2), (T * Hq, s_stride, D)
     int64_t num_pages, table_stride, q_st, q_sh, o_st, o_sh;
     int32_t T, R, width, Hq, Hkv, rep, d, page_shift, top, S, s_stride, chunk, mode, many, units;
+    int32_t q_vec, o_vec;                     // rows of q in 16-byte pieces, of out in 4 elements
     float scale;                              // softmax scale * log2(e)
 };
 
@@ -110,6 +113,17 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// A matrix operand's lane l holds row l % 16 and piece l / 16 of its columns, so
+// neighbouring lanes' pieces lie a whole row apart, and the L1 serves 16 bytes of a
+// row an access where it could serve 64 (measured: 45 accesses a load, its data path
+// 93% busy at 11 TB/s).  Loads therefore go out with piece l % 4 of row l / 4, and the
+// pieces change lanes through LDS: they are written to slot_of(row, piece), read back
+// from slot_of(own row, own piece).  The exclusive or keeps 16-byte accesses free of
+// bank conflicts (counted): writes go 8 neighbouring lanes at a time, two rows' four
+// pieces; reads 16 at a time, half of them 4 lanes in every 12 of one piece, the rest
+// their complement in the next.
+__device__ __forceinline__ int slot_of(int row, int piece) { return piece * 16 + (row ^ (piece << 1)); }
+
 // Matrix operands by the queries' type.  Queries are exact: bf16, f16, or three bf16
 // terms of an fp32.  Probabilities: f16, or three bf16 terms.
 template <typename T> struct Ops {                      // bf16
@@ -184,19 +198,36 @@ struct Columns {
         for (int rt = 0; rt < RT; ++rt) {
             const int c = c0 + rt * 16 + col;
             const bool live = c < c1;
-            const int t = u.t0 + c / p.rep;
-            const int seen = live && u.req >= 0 && p.requests[t] == u.req ? p.positions[t] : -1;
+            // dead lanes load the last live column, so that no load waits for another
+            const int cc = min(c, c1 - 1), t = u.t0 + cc / p.rep;
+            const int32_t req = p.requests[t], at = p.positions[t];
+            const int seen = live && u.req >= 0 && req == u.req ? at : -1;
             most = max(most, seen);
             if (live) least = min(least, seen);
             pos[rt] = live ? seen : 0x7fffffff;
-            const T *row = (const T *)p.q + t * p.q_st + (int64_t)(h * p.rep + c % p.rep) * p.q_sh;
+            const T *row = (const T *)p.q + t * p.q_st + (int64_t)(h * p.rep + cc % p.rep) * p.q_sh;
+            T raw[DP * 2][8];
+            if (p.q_vec) {
+#pragma unroll
+                for (int s = 0; s < DP * 2; ++s) {
+                    const int x = (s >> 1) * 64 + g * 16 + (s & 1) * 8;
+                    __builtin_memcpy(raw[s], __builtin_assume_aligned(row + (x < p.d ? x : 0), 16),
+                                     sizeof(raw[s]));
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < DP * 2; ++s)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        raw[s][j] = row[min((s >> 1) * 64 + g * 16 + (s & 1) * 8 + j, p.d - 1)];
+            }
 #pragma unroll
             for (int s = 0; s < DP * 2; ++s)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int x = (s >> 1) * 64 + g * 16 + (s & 1) * 8 + j;
-                    float v = live && x < p.d ? to_f32(row[x]) : 0.f;
-                    if (neg) v = -v;
+                    float v = to_f32(raw[s][j]);
+                    v = live && x < p.d ? (neg ? -v : v) : 0.f;
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) {
                         const typename O_::QE b = (typename O_::QE)v;
@@ -308,12 +339,22 @@ struct Columns {
                 T *row = (T *)p.out + t * p.o_st + hq * p.o_sh;
                 const float f = sum == 0.f ? 0.f : un / sum;
 #pragma unroll
-                for (int i = 0; i < ND; ++i)
+                for (int i = 0; i < ND; ++i) {
+                    const int x = i * 16 + 4 * g;
+                    T v[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int x = i * 16 + 4 * g + r;
-                        if (x < p.d) Cvt<T>::store(row + x, sum == 0.f ? 0.f : o[rt][i][r] * f);
+                    for (int r = 0; r < 4; ++r)
+                        Cvt<T>::store(v + r, sum == 0.f ? 0.f : o[rt][i][r] * f);
+                    if (p.o_vec) {
+                        if (x < p.d)
+                            __builtin_memcpy(__builtin_assume_aligned(row + x, 4 * sizeof(T)), v,
+                                             sizeof(v));
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (x + r < p.d) row[x + r] = v[r];
                     }
+                }
             } else {
                 const int64_t at = ((int64_t)t * p.Hq + hq) * p.s_stride + split;
                 if (any) {

@@ -6,8 +6,7 @@
 // Here each wave owns 16 RT columns and walks every key tile of the workgroup's
 // range, so the tiles are shared: the waves convert a tile's codes to 16-bit floats
 // once, into LDS, in the order in which the matrix operands read them (a fragment is
-// 64 lanes x 16 bytes: every LDS access is a whole row of banks), double-buffered,
-// with the next tile's codes already on their way from memory.  Bound by the matrix
+// 64 slots of 16 bytes: every LDS access is free of conflicts), double-buffered, with the next tile's codes already on their way from memory.  Bound by the matrix
 // pipe and the exponentials together.
 #include "ssa_cache_attend_dev.h"
 
@@ -23,10 +22,11 @@ cache_prompt_kernel(AttendParams p) {
     constexpr int CT = ATT_WAVES * 16 * RT;
     // a load unit: 16 codes a lane, two fragments
     constexpr int KU = NB * DP, VU = ND * KS / 2, NU = KU + VU, UW = NU / ATT_WAVES;
-    __shared__ uint4 frag[2][2 * NU][SSA_WAVE];
+    __shared__ u32x4 frag[2][2 * NU][SSA_WAVE];
     __shared__ int most_lds[ATT_WAVES];
 
-    const int lane = lane_id(), col = lane & 15, g = lane >> 4;
+    const int lane = lane_id(), lrow = lane >> 2, lpiece = lane & 3;
+    const int to = slot_of(lrow, lpiece), from = slot_of(lane & 15, lane >> 4);
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / SSA_WAVE);
     // kv heads run fastest: an XCD's workgroups share their heads' pages in its L2;
     // units run backwards, those with the most keys first
@@ -52,17 +52,17 @@ cache_prompt_kernel(AttendParams p) {
 
     // this wave's load units: key block b, columns 64 i.. ; or value rows
     int off[UW];
-    uint4 raw[UW];
+    u32x4 raw[UW];
 #pragma unroll
     for (int x = 0; x < UW; ++x) {
         const int un_ = wave * UW + x;
         if (un_ < KU) {
             const int b = un_ / DP, i = un_ % DP;
-            off[x] = (KT / 4 * (col >> 2) + 4 * b + (col & 3)) * D + i * 64 + g * 16;
+            off[x] = (KT / 4 * (lrow >> 2) + 4 * b + (lrow & 3)) * D + i * 64 + lpiece * 16;
         } else {
             const int i = un_ - KU;
-            off[x] = KT == 64 ? ((i * 16 + col) << p.page_shift) + 16 * g
-                              : ((i * 32 + col) << p.page_shift) + 8 * g;
+            off[x] = KT == 64 ? ((i * 16 + lrow) << p.page_shift) + 16 * lpiece
+                              : ((i * 32 + lrow) << p.page_shift) + 8 * lpiece;
         }
     }
     struct Tile { int pg; float ks, vs; };
@@ -84,13 +84,13 @@ cache_prompt_kernel(AttendParams p) {
 #pragma unroll
         for (int x = 0; x < UW; ++x) {
             if (wave * UW + x < KU) {
-                raw[x] = *(const uint4 *)(kb + off[x]);
+                raw[x] = *(const u32x4 *)(kb + off[x]);
             } else if (KT == 64) {
-                raw[x] = *(const uint4 *)(vb + off[x]);
+                raw[x] = *(const u32x4 *)(vb + off[x]);
             } else {
-                const uint2 a = *(const uint2 *)(vb + off[x]);
-                const uint2 b = *(const uint2 *)(vb + off[x] + (16 << p.page_shift));
-                raw[x] = uint4{a.x, a.y, b.x, b.y};
+                const u32x2 a = *(const u32x2 *)(vb + off[x]);
+                const u32x2 b = *(const u32x2 *)(vb + off[x] + (16 << p.page_shift));
+                raw[x] = u32x4{a.x, a.y, b.x, b.y};
             }
         }
     };
@@ -100,11 +100,11 @@ cache_prompt_kernel(AttendParams p) {
         for (int x = 0; x < UW; ++x) {
             const int f = 2 * (wave * UW + x);
             if (wave * UW + x < KU) {
-                *(QV *)&frag[buf][f][lane] = Ops<T>::key(raw[x].x, raw[x].y);
-                *(QV *)&frag[buf][f + 1][lane] = Ops<T>::key(raw[x].z, raw[x].w);
+                *(QV *)&frag[buf][f][to] = Ops<T>::key(raw[x].x, raw[x].y);
+                *(QV *)&frag[buf][f + 1][to] = Ops<T>::key(raw[x].z, raw[x].w);
             } else {
-                *(PV *)&frag[buf][f][lane] = Ops<T>::value(raw[x].x, raw[x].y, ti.vs);
-                *(PV *)&frag[buf][f + 1][lane] = Ops<T>::value(raw[x].z, raw[x].w, ti.vs);
+                *(PV *)&frag[buf][f][to] = Ops<T>::value(raw[x].x, raw[x].y, ti.vs);
+                *(PV *)&frag[buf][f + 1][to] = Ops<T>::value(raw[x].z, raw[x].w, ti.vs);
             }
         }
     };
@@ -135,7 +135,7 @@ cache_prompt_kernel(AttendParams p) {
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int k = 0; k < DP * 2; ++k) {
-                    const QV kf = *(const QV *)&frag[buf][b * DP * 2 + k][lane];
+                    const QV kf = *(const QV *)&frag[buf][b * DP * 2 + k][from];
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -147,7 +147,7 @@ cache_prompt_kernel(AttendParams p) {
             for (int i = 0; i < ND; ++i)
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                    const PV vf = *(const PV *)&frag[buf][2 * KU + i * KS + k][lane];
+                    const PV vf = *(const PV *)&frag[buf][2 * KU + i * KS + k][from];
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
