@@ -42,16 +42,28 @@ def store_dim(d_head: int) -> int:
     return 64 if d_head <= 64 else 128 if d_head <= 128 else 256
 
 
-def _need(cond, what, msg):
-    if not cond:
-        raise RuntimeError(f"ssa_amd.{what}: {msg}")
+# The checks below run on every call of a few microseconds: messages are formed only
+# where one fails.
+def _refuse(what, msg):
+    raise RuntimeError(f"ssa_amd.{what}: {msg}")
 
 
 def _ints(t, name, shape, what, dtype=torch.int32):
     """Raise unless t is a contiguous integer tensor of this shape."""
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
-        raise RuntimeError(f"ssa_amd.{what}: {name} must be a contiguous {dtype} tensor of shape "
-                           f"{tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+        _refuse(what, f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got "
+                f"{t.dtype} {tuple(t.shape)}")
+
+
+def _table(bt, what):
+    """(R, width, elements between rows) of a block table."""
+    if bt.dim() != 2 or bt.dtype != torch.int32:
+        _refuse(what, f"block_table must be 2-D int32, got {bt.dtype} {tuple(bt.shape)}")
+    (R, width), (step, unit) = bt.shape, bt.stride()
+    if R < 1 or width < 1 or (unit != 1 and width > 1) or (step < width and R > 1):
+        _refuse(what, f"block_table {tuple(bt.shape)} must have rows of unit stride, got strides "
+                f"{bt.stride()}")
+    return R, width, step if step > width else width
 
 
 def _one_device(what, dev, *tensors):
@@ -63,15 +75,19 @@ def _one_device(what, dev, *tensors):
 
 
 def _inference(what, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"ssa_amd.{what} is inference only: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                _refuse(what, "inference only: call it under torch.no_grad()")
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on(dev):
     """The device made current for a launch (nothing to do where it is)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+    i = dev.index
+    return _HERE if i is None or i == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 # ---------------------------------------------------------------------------- cache
@@ -106,24 +122,20 @@ class PagedKVCache:
 
     def _set(self, k_codes, v_codes, bounds, k_scale, v_scale, d_head):
         what, D = "PagedKVCache", store_dim(d_head)
-        _need(k_codes.dim() == 4 and k_codes.shape[3] == D, what,
-              f"k_codes {tuple(k_codes.shape)} are not (pages, kv heads, page, {D})")
+        if k_codes.dim() != 4 or k_codes.shape[3] != D:
+            _refuse(what, f"k_codes {tuple(k_codes.shape)} are not (pages, kv heads, page, {D})")
         P, H, ps, _ = k_codes.shape
-        _need(P >= 1 and H >= 1 and ps in PAGE_SIZES, what,
-              f"{P} pages of {ps} tokens, {H} kv heads (pages of 32, 64 or 128 tokens)")
-        for t, shape, name in ((k_codes, (P, H, ps, D), "k_codes"),
-                               (v_codes, (P, H, D, ps), "v_codes"),
-                               (bounds, (P, H, 2, D), "bounds")):
-            if t.shape != shape or t.dtype != E4M3 or not t.is_contiguous():
-                raise RuntimeError(f"ssa_amd.{what}: {name} must be contiguous {E4M3} {shape}, "
-                                   f"got {t.dtype} {tuple(t.shape)}")
-        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-            if t.shape != (P, H) or t.dtype != torch.float32 or not t.is_contiguous():
-                raise RuntimeError(f"ssa_amd.{what}: {name} must be contiguous float32 {(P, H)}, "
-                                   f"got {t.dtype} {tuple(t.shape)}")
-        dev = k_codes.device
-        for t in (v_codes, bounds, k_scale, v_scale):
-            _need(t.device == dev, what, f"buffers on {dev} and {t.device}")
+        if P < 1 or H < 1 or ps not in PAGE_SIZES:
+            _refuse(what, f"{P} pages of {ps} tokens, {H} kv heads (pages of 32, 64 or 128 tokens)")
+        dev, n = k_codes.device, (P, H)
+        for t, shape, dt, name in ((k_codes, (P, H, ps, D), E4M3, "k_codes"),
+                                   (v_codes, (P, H, D, ps), E4M3, "v_codes"),
+                                   (bounds, (P, H, 2, D), E4M3, "bounds"),
+                                   (k_scale, n, torch.float32, "k_scale"),
+                                   (v_scale, n, torch.float32, "v_scale")):
+            if t.shape != shape or t.dtype != dt or t.device != dev or not t.is_contiguous():
+                _refuse(what, f"{name} must be contiguous {dt} {shape} on {dev}, got {t.dtype} "
+                        f"{tuple(t.shape)} on {t.device}")
         self.k_codes, self.v_codes, self.bounds = k_codes, v_codes, bounds
         self.k_scale, self.v_scale = k_scale, v_scale
         self.num_pages, self.num_kv_heads, self.page_size, self.d_head = P, H, ps, d_head
@@ -160,36 +172,32 @@ def plan_pages(cached, new_rows, block_table, free_pages, free_count, *, page_si
     is refused, as a whole, when its rows pass num_rows, its tokens pass width
     pages, a length is negative, or the free pages do not reach it."""
     what = "plan_pages"
-    _need(cached.dim() == 1 and block_table.dim() == 2 and free_pages.dim() == 1, what,
-          f"cached {tuple(cached.shape)}, block_table {tuple(block_table.shape)}, free_pages "
-          f"{tuple(free_pages.shape)}")
-    R, width = block_table.shape
-    _need(R >= 1 and width >= 1 and num_rows >= 0, what,
-          f"{R} requests of {width} pages, {num_rows} rows")
+    R, width, step = _table(block_table, what)
+    if num_rows < 0:
+        _refuse(what, f"{num_rows} rows")
     _ints(cached, "cached", (R,), what)
     _ints(new_rows, "new_rows", (R,), what)
+    if free_pages.dim() != 1:
+        _refuse(what, f"free_pages {tuple(free_pages.shape)}")
     _ints(free_pages, "free_pages", free_pages.shape, what)
     _ints(free_count, "free_count", (1,), what)
-    _need(block_table.dtype == torch.int32 and block_table.stride(1) == 1
-          and (R == 1 or block_table.stride(0) >= width), what,
-          f"block_table must be int32 rows of unit stride, got {block_table.dtype} strides "
-          f"{block_table.stride()}")
     dev = cached.device
     _one_device(what, dev, new_rows, block_table, free_pages, free_count)
     T = int(num_rows)
-    buf = torch.empty(2 * T + 2 * R + 3, dtype=torch.int32, device=dev)
+    slots = torch.empty(T, dtype=torch.int64, device=dev)
+    buf = slots.new_empty(2 * T + 2 * R + 3, dtype=torch.int32)
     starts, lengths, positions, requests, count, refused = buf.split_with_sizes(
         (R + 1, R, T, T, 1, 1))
-    slots = torch.empty(T, dtype=torch.int64, device=dev)
     p = buf.data_ptr()
+    q = p + 4 * (2 * R + 1)
     a = _lib.PagePlanArgs(
-        cached.data_ptr(), new_rows.data_ptr(), block_table.data_ptr(),
-        max(block_table.stride(0), width), R, width, page_size, T, free_pages.data_ptr(),
-        free_pages.numel(), free_count.data_ptr(), p, p + 4 * (R + 1), slots.data_ptr(),
-        p + 4 * (2 * R + 1), p + 4 * (2 * R + 1 + T), p + 4 * (2 * R + 1 + 2 * T),
-        p + 4 * (2 * R + 2 + 2 * T))
+        cached.data_ptr(), new_rows.data_ptr(), block_table.data_ptr(), step, R, width, page_size,
+        T, free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), p, p + 4 * (R + 1),
+        slots.data_ptr(), q, q + 4 * T, q + 8 * T, q + 8 * T + 4)
     with _on(dev):
-        _lib._check(_lib.lib().ssa_page_plan(ctypes.byref(a), _lib._stream(cached)), what)
+        rc = _lib.lib().ssa_page_plan(ctypes.byref(a), _lib._stream(cached))
+    if rc:
+        _lib._check(rc, what)
     return PagePlan(block_table, starts, requests, positions, slots, lengths, count, refused)
 
 
@@ -201,7 +209,8 @@ class PageTable:
     def __init__(self, max_requests: int, max_pages: int, num_pages: int, page_size: int = 64,
                  device="cuda"):
         z = dict(dtype=torch.int32, device=device)
-        _need(page_size in PAGE_SIZES, "PageTable", f"pages of {page_size} tokens (32, 64 or 128)")
+        if page_size not in PAGE_SIZES:
+            _refuse("PageTable", f"pages of {page_size} tokens (32, 64 or 128)")
         self.page_size, self.num_pages = page_size, num_pages
         self.block_table = torch.full((max_requests, max_pages), -1, **z)
         self.lengths = torch.zeros(max_requests, **z)
@@ -235,7 +244,8 @@ class PageTable:
 
 # ---------------------------------------------------------------------------- append
 def _rows3(t, name, what):
-    _need(t.dim() == 3, what, f"{name} must be 3-D (rows, heads, d), got {tuple(t.shape)}")
+    if t.dim() != 3:
+        _refuse(what, f"{name} must be 3-D (rows, heads, d), got {tuple(t.shape)}")
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
@@ -252,44 +262,43 @@ def cache_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
     what = "cache_append"
     k, v = _rows3(k, "k", what), _rows3(v, "v", what)
     T, H, d = k.shape
-    _need(v.shape == k.shape and v.dtype == k.dtype, what,
-          f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ")
-    _need(H == cache.num_kv_heads and d == cache.d_head, what,
-          f"rows of {H} heads of dim {d} into a cache of {cache.num_kv_heads} of dim "
-          f"{cache.d_head}")
+    dt = k.dtype
+    if v.shape != k.shape or v.dtype != dt:
+        _refuse(what, f"k {dt} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ")
+    if H != cache.num_kv_heads or d != cache.d_head:
+        _refuse(what, f"rows of {H} heads of dim {d} into a cache of {cache.num_kv_heads} of dim "
+                f"{cache.d_head}")
     _ints(slots, "slots", (T,), what, torch.int64)
     _inference(what, k, v)
-    dt = _lib.dtype_code(k.dtype)
-    _one_device(what, k.device, v, slots, cache.k_codes)
-    a = _lib.CacheAppendArgs(cache._c, k.data_ptr(), v.data_ptr(), dt, T, k.stride(0), k.stride(1),
-                             v.stride(0), v.stride(1), slots.data_ptr())
-    with _on(k.device):
-        _lib._check(_lib.lib().ssa_cache_append(ctypes.byref(a), _lib._stream(k)), what)
+    code = _lib.dtype_code(dt)
+    dev = k.device
+    _one_device(what, dev, v, slots, cache.k_codes)
+    (k_st, k_sh, _), (v_st, v_sh, _) = k.stride(), v.stride()
+    a = _lib.CacheAppendArgs(cache._c, k.data_ptr(), v.data_ptr(), code, T, k_st, k_sh, v_st, v_sh,
+                             slots.data_ptr())
+    with _on(dev):
+        rc = _lib.lib().ssa_cache_append(ctypes.byref(a), _lib._stream(k))
+    if rc:
+        _lib._check(rc, what)
 
 
 # ---------------------------------------------------------------------------- select, attend
 def _batch(what, q, cache, plan):
-    """Checked (q, ssa_batch_rows) of a batch."""
+    """Checked (q, ssa_batch_rows, T, Hq, d) of a batch."""
     q = _rows3(q, "q", what)
     T, Hq, d = q.shape
-    _need(Hq >= 1 and Hq % cache.num_kv_heads == 0, what,
-          f"{Hq} query heads are not a multiple of {cache.num_kv_heads} kv heads")
-    _need(d == cache.d_head, what, f"q has head dim {d}, the cache {cache.d_head}")
-    bt = plan.block_table
-    _need(bt.dim() == 2 and bt.shape[0] >= 1 and bt.shape[1] >= 1, what,
-          f"block_table {tuple(bt.shape)}")
-    R, width = bt.shape
-    _need(bt.dtype == torch.int32 and bt.stride(1) == 1 and (R == 1 or bt.stride(0) >= width),
-          what, f"block_table must be int32 rows of unit stride, got {bt.dtype} strides "
-          f"{bt.stride()}")
-    _ints(plan.starts, "starts", (R + 1,), what)
-    _ints(plan.requests, "requests", (T,), what)
-    _ints(plan.positions, "positions", (T,), what)
+    if Hq < 1 or Hq % cache.num_kv_heads or d != cache.d_head:
+        _refuse(what, f"q has {Hq} heads of dim {d}, the cache {cache.num_kv_heads} of dim "
+                f"{cache.d_head} (query heads a multiple of kv heads, one head dim)")
+    bt, starts, requests, positions = plan.block_table, plan.starts, plan.requests, plan.positions
+    R, width, step = _table(bt, what)
+    _ints(starts, "starts", (R + 1,), what)
+    _ints(requests, "requests", (T,), what)
+    _ints(positions, "positions", (T,), what)
     _inference(what, q)
-    _one_device(what, q.device, bt, plan.starts, plan.requests, plan.positions, cache.k_codes)
-    return q, _lib.BatchRows(bt.data_ptr(), max(bt.stride(0), width), R, width,
-                             plan.starts.data_ptr(), plan.requests.data_ptr(),
-                             plan.positions.data_ptr(), T)
+    _one_device(what, q.device, bt, starts, requests, positions, cache.k_codes)
+    return q, _lib.BatchRows(bt.data_ptr(), step, R, width, starts.data_ptr(), requests.data_ptr(),
+                             positions.data_ptr(), T), T, Hq, d
 
 
 def select_pages(q: torch.Tensor, cache: PagedKVCache, plan: PagePlan, top_k: int, *,
@@ -300,15 +309,18 @@ def select_pages(q: torch.Tensor, cache: PagedKVCache, plan: PagePlan, top_k: in
     others those with the largest bound of the group's summed scores (ties to
     the lower page).  recent >= 1, first + recent <= top_k."""
     what = "select_pages"
-    _need(first >= 0 and recent >= 1 and first + recent <= top_k, what,
-          f"first={first} recent={recent} top_k={top_k} (recent >= 1, both within top_k)")
-    q, rows = _batch(what, q, cache, plan)
-    T, Hq, _ = q.shape
+    if not (first >= 0 and recent >= 1 and first + recent <= top_k):
+        _refuse(what, f"first={first} recent={recent} top_k={top_k} (recent >= 1, both within "
+                "top_k)")
+    q, rows, T, Hq, _ = _batch(what, q, cache, plan)
     out = torch.empty((T, cache.num_kv_heads, top_k), dtype=torch.int32, device=q.device)
-    a = _lib.SelectPagesArgs(cache._c, rows, q.data_ptr(), _lib.dtype_code(q.dtype), Hq,
-                             q.stride(0), q.stride(1), top_k, first, recent, out.data_ptr())
+    q_st, q_sh, _ = q.stride()
+    a = _lib.SelectPagesArgs(cache._c, rows, q.data_ptr(), _lib.dtype_code(q.dtype), Hq, q_st, q_sh,
+                             top_k, first, recent, out.data_ptr())
     with _on(q.device):
-        _lib._check(_lib.lib().ssa_select_pages(ctypes.byref(a), _lib._stream(q)), what)
+        rc = _lib.lib().ssa_select_pages(ctypes.byref(a), _lib._stream(q))
+    if rc:
+        _lib._check(rc, what)
     return out
 
 
@@ -322,31 +334,33 @@ def cached_attention(q: torch.Tensor, cache: PagedKVCache, plan: PagePlan, *,
     (padding, a refused request) get zeros.  Returns (T, Hq, d_head) in q's
     dtype (`out`, where given)."""
     what = "cached_attention"
-    q, rows = _batch(what, q, cache, plan)
-    T, Hq, d = q.shape
+    q, rows, T, Hq, d = _batch(what, q, cache, plan)
+    dev = q.device
     top, pp = 0, None
     if pages is not None:
-        _need(pages.dim() == 3 and pages.shape[2] >= 1, what, f"pages {tuple(pages.shape)}")
+        if pages.dim() != 3 or pages.shape[2] < 1:
+            _refuse(what, f"pages {tuple(pages.shape)} are not (rows, kv heads, pages)")
         top = pages.shape[2]
         _ints(pages, "pages", (T, cache.num_kv_heads, top), what)
-        _one_device(what, q.device, pages)
+        _one_device(what, dev, pages)
         pp = pages.data_ptr()
     if out is None:
-        out = torch.empty((T, Hq, d), dtype=q.dtype, device=q.device)
-    else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device
-              and (out.stride(2) == 1 or d == 1), what,
-              f"out {out.dtype} {tuple(out.shape)} does not fit q {q.dtype} {tuple(q.shape)}")
+        out = torch.empty((T, Hq, d), dtype=q.dtype, device=dev)
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != dev
+          or (out.stride(2) != 1 and d > 1)):
+        _refuse(what, f"out {out.dtype} {tuple(out.shape)} strides {out.stride()} does not fit q "
+                f"{q.dtype} {tuple(q.shape)}")
+    (q_st, q_sh, _), (o_st, o_sh, _) = q.stride(), out.stride()
     a = _lib.CachedAttentionArgs(cache._c, rows, q.data_ptr(), out.data_ptr(),
-                                 _lib.dtype_code(q.dtype), Hq, q.stride(0), q.stride(1),
-                                 out.stride(0), out.stride(1),
+                                 _lib.dtype_code(q.dtype), Hq, q_st, q_sh, o_st, o_sh,
                                  d ** -0.5 if scale is None else float(scale), pp, top)
-    L = _lib.lib()
-    with _on(q.device):
-        n = L.ssa_cached_attention_workspace_bytes(ctypes.byref(a))
+    L, ref = _lib.lib(), ctypes.byref(a)
+    with _on(dev):
+        n = L.ssa_cached_attention_workspace_bytes(ref)
         if n < 0:
             _lib._check(int(n), what)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        _lib._check(L.ssa_cached_attention(ctypes.byref(a), None if ws is None else ws.data_ptr(),
-                                           n, _lib._stream(q)), what)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        rc = L.ssa_cached_attention(ref, ws.data_ptr() if n else None, n, _lib._stream(q))
+    if rc:
+        _lib._check(rc, what)
     return out
