@@ -41,6 +41,8 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *part, uint3
     return sat_add(before, lane == 0 ? 0u : own);
 }
 
+// PER: requests of a thread, held in registers between the scans
+template <int PER>
 __global__ void __launch_bounds__(PLAN_THREADS)
 page_plan_kernel(ssa_page_plan_args a) {
     extern __shared__ uint32_t plan_lds[];
@@ -48,38 +50,49 @@ page_plan_kernel(ssa_page_plan_args a) {
     __shared__ uint32_t n_taken, n_refused;
     uint32_t *end = plan_lds;               // rows up to and with request r
     int32_t *base = (int32_t *)plan_lds + a.R;   // pages taken before r, -1 where refused
-    const int per = (a.R + PLAN_THREADS - 1) / PLAN_THREADS;
-    const int r0 = min((int)threadIdx.x * per, a.R), r1 = min(r0 + per, a.R);
+    const int r0 = (int)threadIdx.x * PER;
     const bool first_wg = blockIdx.x == 0;
     if (threadIdx.x == 0) n_taken = n_refused = 0;
+    int c[PER], n[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {          // all in flight at once
+        const int r = min(r0 + i, a.R - 1);
+        c[i] = a.cached[r];
+        n[i] = a.new_rows[r];
+    }
+    const uint32_t nfree = (uint32_t)max(0, min(*a.free_count, a.free_capacity));
     uint32_t sum = 0, total;
-    for (int r = r0; r < r1; ++r) sum = sat_add(sum, (uint32_t)max(a.new_rows[r], 0));
-    uint32_t run = block_scan(sum, part, &total);
-    uint32_t need = 0;
-    for (int r = r0; r < r1; ++r) {
-        const int c = a.cached[r], n = a.new_rows[r];
-        if (first_wg) a.starts[r] = (int32_t)run;
-        run = sat_add(run, (uint32_t)max(n, 0));
-        end[r] = run;
-        const int64_t want = ((int64_t)c + n + a.page - 1) / a.page;
-        const bool fits = c >= 0 && n >= 0 && want <= a.width && run <= (uint32_t)a.T;
-        const int nd = fits ? (int)(want - ((int64_t)c + a.page - 1) / a.page) : -1;
-        base[r] = nd;
-        need = sat_add(need, (uint32_t)max(nd, 0));
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (r0 + i < a.R) sum = sat_add(sum, (uint32_t)max(n[i], 0));
+    uint32_t run = block_scan(sum, part, &total), need = 0;
+    const int page_shift = 31 - __clz(a.page);
+    int nd[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        nd[i] = -1;
+        if (r0 + i >= a.R) continue;
+        if (first_wg) a.starts[r0 + i] = (int32_t)run;
+        run = sat_add(run, (uint32_t)max(n[i], 0));
+        end[r0 + i] = run;
+        const int64_t want = ((int64_t)c[i] + n[i] + a.page - 1) >> page_shift;
+        const bool fits = c[i] >= 0 && n[i] >= 0 && want <= a.width && run <= (uint32_t)a.T;
+        if (fits) nd[i] = (int)(want - (((int64_t)c[i] + a.page - 1) >> page_shift));
+        need = sat_add(need, (uint32_t)max(nd[i], 0));
     }
     if (first_wg && threadIdx.x == 0) a.starts[a.R] = (int32_t)total;
     uint32_t upto = block_scan(need, part, &total);
-    const uint32_t nfree = (uint32_t)max(0, min(*a.free_count, a.free_capacity));
     uint32_t taken = 0, refused = 0;
-    for (int r = r0; r < r1; ++r) {
-        const int nd = base[r];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (r0 + i >= a.R) continue;
         const uint32_t before = upto;
-        upto = sat_add(upto, (uint32_t)max(nd, 0));
-        const bool ok = nd == 0 || (nd > 0 && upto <= nfree);
-        base[r] = ok ? (int32_t)min(before, nfree) : -1;
-        taken += ok ? (uint32_t)nd : 0u;
+        upto = sat_add(upto, (uint32_t)max(nd[i], 0));
+        const bool ok = nd[i] == 0 || (nd[i] > 0 && upto <= nfree);
+        base[r0 + i] = ok ? (int32_t)min(before, nfree) : -1;
+        taken += ok ? (uint32_t)nd[i] : 0u;
         refused += ok ? 0u : 1u;
-        if (first_wg) a.lengths[r] = a.cached[r] + (ok ? a.new_rows[r] : 0);
+        if (first_wg) a.lengths[r0 + i] = c[i] + (ok ? n[i] : 0);
     }
     __syncthreads();
     if (first_wg) {
@@ -102,11 +115,11 @@ page_plan_kernel(ssa_page_plan_args a) {
         int64_t slot = -1;
         int32_t pos = -1, req = -1;
         if (lo < a.R && base[lo] >= 0) {
-            const int c = a.cached[lo];
+            const int held = a.cached[lo];
             req = lo;
-            pos = c + (int32_t)(t - (lo ? end[lo - 1] : 0));
-            const int col = pos / a.page, off = pos - col * a.page;
-            const int had = (c + a.page - 1) / a.page;
+            pos = held + (int32_t)(t - (lo ? end[lo - 1] : 0));
+            const int col = pos >> page_shift, off = pos & (a.page - 1);
+            const int had = (held + a.page - 1) >> page_shift;
             int32_t *entry = a.block_table + (int64_t)lo * a.table_stride + col;
             int32_t page;
             if (col < had) {
@@ -123,41 +136,77 @@ page_plan_kernel(ssa_page_plan_args a) {
     }
 }
 
+template <int PER>
+int launch_plan(const ssa_page_plan_args &a, hipStream_t s) {
+    const size_t lds = (size_t)a.R * 8;
+    SSA_ALLOW_LDS(page_plan_kernel<PER>, lds);
+    // a thread a row: the scans are repeated side by side, rows would be in turn
+    const int64_t want = ceil_div(a.T, PLAN_THREADS);
+    const int grid = (int)(want < 1 ? 1 : (want > 1024 ? 1024 : want));
+    page_plan_kernel<PER><<<grid, PLAN_THREADS, lds, s>>>(a);
+    return SSA_OK;
+}
+
 // ---------------------------------------------------------------------------- append
 // One workgroup per run of adjacent rows of one page and kv head: the run's
 // largest magnitudes first (the page's scale has to hold before any code is
 // rounded), then the codes, staged in LDS so that the transposed value codes go
-// out 16 tokens at a time.  D / 8 lanes hold a row, 8 columns each; every row is
-// read twice, the second time from the L2.  Bound by latency for single tokens
-// (about five dependent steps), by reading and writing HBM for prompts.
-constexpr int APP_THREADS = 256;
+// out 16 tokens at a time.  D / 8 lanes hold a row, 8 columns each, and keep it in
+// registers between the two.  Bound by latency for single tokens (about five
+// dependent steps), by reading and writing HBM for prompts.
+
+// Eight adjacent columns of a row, in the registers they take as they are stored.
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+template <typename T> struct Row8 {                        // 16-bit types
+    u32x4 w;
+    __device__ __forceinline__ float get(int j) const {
+        T t;
+        t.x = (uint16_t)(w[j >> 1] >> 16 * (j & 1));
+        return to_f32(t);
+    }
+    __device__ __forceinline__ void set(int j, T t) {
+        w[j >> 1] = j & 1 ? (w[j >> 1] & 0xffffu) | (uint32_t)t.x << 16 : (uint32_t)t.x;
+    }
+    __device__ __forceinline__ void load(const T *p) { w = *(const u32x4 *)p; }
+    __device__ __forceinline__ void clear() { w = u32x4{0, 0, 0, 0}; }
+};
+template <> struct Row8<float> {
+    u32x4 w[2];
+    __device__ __forceinline__ float get(int j) const { return __uint_as_float(w[j >> 2][j & 3]); }
+    __device__ __forceinline__ void set(int j, float t) { w[j >> 2][j & 3] = __float_as_uint(t); }
+    __device__ __forceinline__ void load(const float *p) {
+        w[0] = *(const u32x4 *)p;
+        w[1] = *(const u32x4 *)(p + 4);
+    }
+    __device__ __forceinline__ void clear() { w[0] = w[1] = u32x4{0, 0, 0, 0}; }
+};
 
 // columns x .. x + 7 of a row, zeros past d.  VEC: d and the strides are multiples
 // of 8 (the addresses of 16 bytes)
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_row8(const void *p, int64_t at, int x, int d, float (&v)[8]) {
-    const T *q = (const T *)p + at + x;
+__device__ __forceinline__ void load_row8(const void *p, int64_t at, int x, int d, Row8<T> &v) {
+    const T *q = (const T *)p + at;
     if (VEC) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.f;
-        if (x < d) {
-            T t[8];
-            __builtin_memcpy(t, __builtin_assume_aligned(q, 16), sizeof(t));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = to_f32(t[j]);
-        }
+        v.load(q + (x < d ? x : 0));
+        if (x >= d) v.clear();
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = x + j < d ? to_f32(q[j]) : 0.f;
+        for (int j = 0; j < 8; ++j) v.set(j, x + j < d ? q[x + j] : T{});
     }
 }
 
 // bits of the largest magnitude; a NaN's, its sign cleared, pass every number's
-__device__ __forceinline__ uint32_t max_bits8(const float (&v)[8]) {
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits8(const Row8<T> &v) {
     uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v.get(j)) & 0x7fffffffu);
     return m;
+}
+template <typename T>
+__device__ __forceinline__ uint2 codes8(const Row8<T> &v, float f) {
+    return uint2{codes4(v.get(0) * f, v.get(1) * f, v.get(2) * f, v.get(3) * f),
+                 codes4(v.get(4) * f, v.get(5) * f, v.get(6) * f, v.get(7) * f)};
 }
 
 // smallest e with a <= 448 * 2^e: 448 = 1.75 * 2^8
@@ -175,10 +224,11 @@ __device__ __forceinline__ int code_rank(uint32_t code) {
     return (code & 0x80u) ? -(int)(code & 0x7fu) : (int)(code & 0x7fu);
 }
 
-template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(APP_THREADS)
+template <typename T, int D, bool VEC, int APP_THREADS>
+__global__ void __launch_bounds__(APP_THREADS, sizeof(T) == 4 || !VEC ? 2 : 3)
 cache_append_kernel(ssa_cache_append_args a, int window) {
     constexpr int LPR = D / 8, RPW = APP_THREADS / LPR;   // lanes of a row, rows at a time
+    constexpr int ROWS = 128 / RPW;                       // a thread's share of the most rows
     extern __shared__ uint4 app_lds[];
     __shared__ uint32_t kmax[128], vmax[128];     // bits of each row's largest magnitude
     __shared__ uint32_t page_max[2], any_bad;
@@ -191,28 +241,28 @@ cache_append_kernel(ssa_cache_append_args a, int window) {
 
     // the window's first rows of runs: every wave finds them for itself
     const int64_t w0 = (int64_t)blockIdx.x * window;
-    int64_t mine = -1;
-    bool first = false;
-    if (lane < window && w0 + lane < a.T) {
-        mine = a.slots[w0 + lane];
-        const int64_t prev = w0 + lane > 0 ? a.slots[w0 + lane - 1] : -1;
-        first = mine >= 0 && mine < cap && (mine % ps == 0 || prev != mine - 1);
-    }
+    int64_t at[3];                                // slots of rows w0 + lane, + 64, + 128
+#pragma unroll
+    for (int i = 0; i < 3; ++i) at[i] = w0 + 64 * i + lane < a.T ? a.slots[w0 + 64 * i + lane] : -1;
+    const int64_t before = w0 > 0 ? a.slots[w0 - 1] : -1;
+    const int64_t up = __shfl_up(at[0], 1, SSA_WAVE), prev = lane ? up : before;
+    const int page_shift = 31 - __clz(ps);
+    const bool first = lane < window && at[0] >= 0 && at[0] < cap &&
+                       ((at[0] & (ps - 1)) == 0 || prev != at[0] - 1);
     uint64_t todo = wave_ballot(first);
     while (todo) {
         const int w = __ffsll((unsigned long long)todo) - 1;
         todo &= todo - 1;
-        const int64_t t0 = w0 + w, slot = __shfl(mine, w, SSA_WAVE);
-        const int64_t pg = slot / ps;
-        const int off = (int)(slot - pg * ps);
-        // length of the run: rows t0 + i at slot + i within the page
-        const int most = (int)min((int64_t)(ps - off), a.T - t0);
-        int n = 1;
-        for (int b = 0; b < most; b += SSA_WAVE) {
-            const int i = b + lane;
-            const uint64_t m = wave_ballot(i < most && a.slots[t0 + i] == slot + i);
-            n = b + (m == ~0ull ? SSA_WAVE : __ffsll((unsigned long long)~m) - 1);
-            if (m != ~0ull) break;
+        const int64_t t0 = w0 + w, slot = __shfl(at[0], w, SSA_WAVE);
+        const int64_t pg = slot >> page_shift;
+        const int off = (int)slot & (ps - 1);
+        // length of the run: rows w0 + j at slot + j - w, within the page
+        int n = ps - off;
+#pragma unroll
+        for (int i = 2; i >= 0; --i) {
+            const int j = 64 * i + lane;
+            const uint64_t m = wave_ballot(j > w && at[i] != slot + j - w);
+            if (m) n = min(n, 64 * i + __ffsll((unsigned long long)m) - 1 - w);
         }
         const int64_t ph = pg * c.Hkv + h;
         const float k_old = off ? c.k_scale[ph] : 0.f, v_old = off ? c.v_scale[ph] : 0.f;
@@ -221,31 +271,27 @@ cache_append_kernel(ssa_cache_append_args a, int window) {
         __syncthreads();                                   // the last run's LDS is read
         if (tid < 2) page_max[tid] = 0;
         if (tid == 2) any_bad = 0;
-        for (int b = r0; b - r0 < n; b += 4 * RPW) {       // four rows in flight
-            uint32_t km[4], vm[4];
+        Row8<T> kv[ROWS], vv[ROWS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = b + i * RPW;
-                float kv[8] = {}, vv[8] = {};
-                if (r < n) {
-                    load_row8<T, VEC>(a.k, krow + r * a.k_st, rx, d, kv);
-                    load_row8<T, VEC>(a.v, vrow + r * a.v_st, rx, d, vv);
-                }
-                km[i] = max_bits8(kv);
-                vm[i] = max_bits8(vv);
+        for (int i = 0; i < ROWS; ++i) {
+            const int r = min(r0 + i * RPW, n - 1);        // past the run: its last row again
+            if (i > 0 && i * RPW >= n) break;
+            load_row8<T, VEC>(a.k, krow + r * a.k_st, rx, d, kv[i]);
+            load_row8<T, VEC>(a.v, vrow + r * a.v_st, rx, d, vv[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            if (i > 0 && i * RPW >= n) break;
+            uint32_t km = max_bits8(kv[i]), vm = max_bits8(vv[i]);
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) {
+                km = max(km, (uint32_t)__shfl_xor((int)km, o, SSA_WAVE));
+                vm = max(vm, (uint32_t)__shfl_xor((int)vm, o, SSA_WAVE));
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                for (int o = LPR / 2; o > 0; o >>= 1) {
-                    km[i] = max(km[i], (uint32_t)__shfl_xor((int)km[i], o, SSA_WAVE));
-                    vm[i] = max(vm[i], (uint32_t)__shfl_xor((int)vm[i], o, SSA_WAVE));
-                }
-                const int r = b + i * RPW;
-                if (rx == 0 && r < n) {
-                    kmax[r] = km[i];
-                    vmax[r] = vm[i];
-                }
+            const int r = r0 + i * RPW;
+            if (rx == 0 && r < n) {
+                kmax[r] = km;
+                vmax[r] = vm;
             }
         }
         __syncthreads();
@@ -296,20 +342,14 @@ cache_append_kernel(ssa_cache_append_args a, int window) {
             hi_lds[x] = hi;
         }
         const float ki = 1.f / k_new, vi = 1.f / v_new;    // exact
-#pragma unroll 4
-        for (int r = r0; r < n; r += RPW) {
-            float kv[8], vv[8];
-            load_row8<T, VEC>(a.k, krow + r * a.k_st, rx, d, kv);
-            load_row8<T, VEC>(a.v, vrow + r * a.v_st, rx, d, vv);
-            const bool bad = kmax[r] == 0xffffffffu;
-            uint2 kc, vc;
-            kc.x = codes4(kv[0] * ki, kv[1] * ki, kv[2] * ki, kv[3] * ki);
-            kc.y = codes4(kv[4] * ki, kv[5] * ki, kv[6] * ki, kv[7] * ki);
-            vc.x = codes4(vv[0] * vi, vv[1] * vi, vv[2] * vi, vv[3] * vi);
-            vc.y = codes4(vv[4] * vi, vv[5] * vi, vv[6] * vi, vv[7] * vi);
-            if (bad) {
-                kc.x = kc.y = SSA_CODE_NAN * 0x01010101u;
-                vc.x = vc.y = 0;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int r = r0 + i * RPW;
+            if (r >= n) break;
+            uint2 kc = codes8(kv[i], ki), vc = codes8(vv[i], vi);
+            if (kmax[r] == 0xffffffffu) {                  // a row that is not finite
+                kc = uint2{SSA_CODE_NAN * 0x01010101u, SSA_CODE_NAN * 0x01010101u};
+                vc = uint2{0, 0};
             }
             *(uint2 *)(kst + r * D + rx) = kc;
             *(uint2 *)(vst + r * D + rx) = vc;
@@ -392,25 +432,29 @@ cache_append_kernel(ssa_cache_append_args a, int window) {
     }
 }
 
-template <typename T, int D>
-int launch_append(const ssa_cache_append_args &a, hipStream_t s) {
-    // a workgroup looks at `window` rows for the first rows of runs: one each while
-    // every row may be one (single tokens: a run each), more where most lie inside
-    const int window = a.T <= 1024 ? 1 : (a.T <= 4096 ? 4 : 16);
+template <typename T, int D, bool VEC, int NT>
+int launch_append_nt(const ssa_cache_append_args &a, int window, hipStream_t s) {
     const dim3 grid((unsigned)ceil_div(a.T, window), (unsigned)a.cache.Hkv);
     const size_t lds = (size_t)2 * a.cache.page * D;
+    SSA_ALLOW_LDS((cache_append_kernel<T, D, VEC, NT>), lds);
+    cache_append_kernel<T, D, VEC, NT><<<grid, NT, lds, s>>>(a, window);
+    return SSA_OK;
+}
+
+template <typename T, int D>
+int launch_append(const ssa_cache_append_args &a, hipStream_t s) {
+    // a workgroup looks at `window` rows for the first rows of runs and serves them in
+    // turn: about 1,024 workgroups in all, what the chip holds at once, whether each
+    // row is a run (single tokens) or most lie inside one (prompts)
+    const int64_t per = (int64_t)a.T * a.cache.Hkv / 1024;
+    const int window = (int)(per < 1 ? 1 : (per > SSA_WAVE ? SSA_WAVE : per));
     // rows in 16-byte pieces (8 elements) where they all start at one
     const int64_t strides = a.k_st | a.k_sh | a.v_st | a.v_sh;
     const bool vec = a.cache.d % 8 == 0 && (strides * (int64_t)sizeof(T)) % 16 == 0 &&
                      (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0;
-    if (vec) {
-        SSA_ALLOW_LDS((cache_append_kernel<T, D, true>), lds);
-        cache_append_kernel<T, D, true><<<grid, APP_THREADS, lds, s>>>(a, window);
-    } else {
-        SSA_ALLOW_LDS((cache_append_kernel<T, D, false>), lds);
-        cache_append_kernel<T, D, false><<<grid, APP_THREADS, lds, s>>>(a, window);
-    }
-    return SSA_OK;
+    constexpr int NT = D == 256 ? 512 : 256;   // at most 8 rows a thread
+    return vec ? launch_append_nt<T, D, true, NT>(a, window, s)
+               : launch_append_nt<T, D, false, NT>(a, window, s);
 }
 
 template <typename T>
@@ -480,14 +524,19 @@ select_pages_kernel(ssa_select_pages_args a) {
         min_hi = ~0u;
     }
     __syncthreads();
+    if (PARTS > 1) {
+        if (tid < 2 * D) {
+            double v = qsum[tid];
+#pragma unroll
+            for (int i = 1; i < PARTS; ++i) v += qsum[i * 2 * D + tid];
+            qsum[tid] = v;
+        }
+        __syncthreads();
+    }
     const int sub = tid % LP;
     double qr[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        qr[j] = qsum[sub * 16 + j];
-#pragma unroll
-        for (int i = 1; i < PARTS; ++i) qr[j] += qsum[i * 2 * D + sub * 16 + j];
-    }
+    for (int j = 0; j < 16; ++j) qr[j] = qsum[sub * 16 + j];
     const int first = min(a.first, n), last = max(n - a.recent, first);
     const int32_t *table = a.rows.block_table + (int64_t)r * a.rows.table_stride;
     uint32_t mx = 0, mn = ~0u;
@@ -667,12 +716,12 @@ extern "C" int ssa_page_plan(const ssa_page_plan_args *a, void *stream) {
                       a->lengths && a->free_count_out && a->refused &&
                       (a->T == 0 || (a->slots && a->positions && a->requests)),
                   "page_plan: null pointer");
-    const size_t lds = (size_t)a->R * 8;
-    SSA_ALLOW_LDS(page_plan_kernel, lds);
-    // workgroups enough for four rows a thread, at most two per CU
-    const int64_t want = ceil_div(a->T, PLAN_THREADS * 4);
-    const int grid = (int)(want < 1 ? 1 : (want > 512 ? 512 : want));
-    page_plan_kernel<<<grid, PLAN_THREADS, lds, (hipStream_t)stream>>>(*a);
+    const hipStream_t s = (hipStream_t)stream;
+    const int rc = a->R <= PLAN_THREADS       ? launch_plan<1>(*a, s)
+                   : a->R <= 4 * PLAN_THREADS ? launch_plan<4>(*a, s)
+                   : a->R <= 16 * PLAN_THREADS ? launch_plan<16>(*a, s)
+                                               : launch_plan<64>(*a, s);
+    if (rc != SSA_OK) return rc;
     SSA_CHECK_LAUNCH();
     return SSA_OK;
 }

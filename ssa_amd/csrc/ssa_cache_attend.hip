@@ -19,279 +19,76 @@
 
 namespace {
 
-// A unit is 16 RT columns.  SHARED: a workgroup takes one unit and a chunk of its key
-// tiles, its waves every fourth tile, and their sums are joined in LDS.  Otherwise
-// each wave takes a unit of its own and all of its tiles: no joining, for calls with
-// units enough to fill the chip.  A wave holds one tile's values and the next one's
-// keys in flight, and looks page ids up a tile ahead of those.
 template <typename T, int D, int KT, int RT, bool SHARED>
 __global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE, D <= 128 && RT == 1 ? 2 : 1)
 cache_attend_kernel(AttendParams p) {
-    typedef Columns<T, D, KT, RT> C;
-    typedef typename C::PV PV;
-    constexpr int NQ = C::NQ, NP = C::NP, NB = C::NB, DP = C::DP, ND = C::ND, KS = C::KS;
-    constexpr int CT = 16 * RT, OS = D + 4;   // OS: row stride of the joined sums
-    // each wave's pieces on their way to other lanes; then the joined sums
-    constexpr int XW = KT * D / 16, XN = ATT_WAVES * XW, ON = SHARED ? CT * OS / 4 : 0;
-    __shared__ u32x4 x_lds[XN > ON ? XN : ON];
-    float *o_lds = (float *)x_lds;
-    __shared__ float m_lds[ATT_WAVES][CT], l_lds[ATT_WAVES][CT];
-
-    const int lane = lane_id(), col = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / SSA_WAVE);
-    // kv heads run fastest: an XCD's workgroups share their heads' pages in its L2
-    const int h = (int)(blockIdx.x % (unsigned)p.Hkv), split = (int)blockIdx.y;
-    int u = (int)(blockIdx.x / (unsigned)p.Hkv);
-    if (!SHARED) u = u * ATT_WAVES + wave;
-    Unit un;
-    if (u >= p.units || !locate_unit(p, u, CT, un)) return;
-    C w;
-    w.start(p, un, un.c0, un.c1, h);
-
-    const int page = 1 << p.page_shift, sub_shift = p.page_shift - (KT == 64 ? 6 : 5);
-    const int32_t *list = p.pages ? p.pages + ((int64_t)un.t0 * p.Hkv + h) * p.top : nullptr;
-    const int32_t *table = p.table + (int64_t)(un.req < 0 ? 0 : un.req) * p.table_stride;
-    const int n_tiles = w.most < 0 ? 0 : (list ? p.top << sub_shift : w.most / KT + 1);
-    const int tile0 = split * p.chunk, tile1 = min(tile0 + p.chunk, n_tiles);
-    constexpr int STEP = SHARED ? ATT_WAVES : 1;
-
-    // The logical page of a tile and its entry in the table, looked up a tile ahead
-    // of its keys: the loads are unconditional (of some entry that is there) and
-    // what they say is judged only where it is needed, so nothing waits for them.
-    const int last_entry = (max(tile1, 1) - 1) >> sub_shift;
-    auto look_up = [&](int tile) { return list ? list[min(tile >> sub_shift, last_entry)] : tile >> sub_shift; };
-    auto entry = [&](int lp) { return table[max(0, min(lp, p.width - 1))]; };
-    // the page's place in the cache, -1 if it is absent or unseen
-    auto place = [&](int tile, int lp, int pg) {
-        const int key0 = (lp << p.page_shift) + (tile & ((1 << sub_shift) - 1)) * KT;
-        return tile < tile1 && lp >= 0 && lp < p.width && key0 <= w.most && pg >= 0 && pg < p.num_pages
-                   ? pg : -1;
-    };
-    u32x4 *xk = x_lds + wave * XW;            // [block][64 columns][slot]
-    u32x2 *xv = (u32x2 *)xk;                  // pages of 32: [16 columns][slot]
-    const int lrow = lane >> 2, lpiece = lane & 3, to = slot_of(lrow, lpiece), from = slot_of(col, g);
-    u32x4 kr[NB][DP];
-    float ks = 0.f, vs = 0.f;
-    auto fetch_keys = [&](int tile, int pg) {
-        if (pg < 0) return;
-        const int64_t ph = (int64_t)pg * p.Hkv + h;
-        ks = p.ks[ph];
-        vs = p.vs[ph];
-        const uint8_t *kb = p.k + ph * page * D + (int64_t)(tile & ((1 << sub_shift) - 1)) * KT * D;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int i = 0; i < DP; ++i)
-                kr[b][i] = *(const u32x4 *)(kb + (KT / 4 * (lrow >> 2) + 4 * b + (lrow & 3)) * D + i * 64 + lpiece * 16);
-    };
-
-    int tile = tile0 + (SHARED ? wave : 0);
-    int lp = 0, lp1 = 0, pg = -1;
-    if (tile < tile1) {
-        lp = look_up(tile);
-        lp1 = look_up(tile + STEP);
-        pg = place(tile, lp, entry(lp));
-        fetch_keys(tile, pg);
-    }
-    for (; tile < tile1; tile += STEP) {
-        int pg1, lp2;
-        if (pg >= 0) {
-            const int sub = tile & ((1 << sub_shift) - 1);
-            const float kscale = ks, vscale = vs;
-            const uint8_t *vb = p.v + ((int64_t)pg * p.Hkv + h) * D * page + sub * KT;
-            uint32_t vr[ND][KT / 16];
-#pragma unroll
-            for (int i = 0; i < ND; ++i) {
-                const uint8_t *at = vb + ((i * 16 + lrow) << p.page_shift) + KT / 4 * lpiece;
-                if constexpr (KT == 64) {
-                    const u32x4 x = *(const u32x4 *)at;
-                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][2] = x.z; vr[i][3] = x.w;
-                } else {
-                    const u32x2 x = *(const u32x2 *)at;
-                    vr[i][0] = x.x; vr[i][1] = x.y;
-                }
-            }
-            // loads go out in this order: values, then what the next tile's need
-            __builtin_amdgcn_sched_barrier(0);
-            const int entry1 = entry(lp1);
-            lp2 = look_up(tile + 2 * STEP);
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < DP; ++i) xk[(b * DP + i) * SSA_WAVE + to] = kr[b][i];
-            wave_lds_sync();
-            f32x4 s[RT][NB];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) s[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < DP; ++i) {
-                    const u32x4 x = xk[(b * DP + i) * SSA_WAVE + from];
-                    const typename C::QV k0 = Ops<T>::key(x.x, x.y), k1 = Ops<T>::key(x.z, x.w);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int n = NQ - 1; n >= 0; --n) {
-                            s[rt][b] = mfma(k0, w.q[rt][2 * i][n], s[rt][b]);
-                            s[rt][b] = mfma(k1, w.q[rt][2 * i + 1][n], s[rt][b]);
-                        }
-                }
-            }
-            pg1 = place(tile + STEP, lp1, entry1);
-            fetch_keys(tile + STEP, pg1);
-            __builtin_amdgcn_sched_barrier(0);
-            PV pf[RT][KS][NP];
-            w.softmax(s, kscale, vscale, (lp << p.page_shift) + sub * KT, pf);
-            wave_lds_sync();
-#pragma unroll
-            for (int i = 0; i < ND; ++i) {
-                if constexpr (KT == 64)
-                    xk[i * SSA_WAVE + to] = u32x4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]};
-                else
-                    xv[i * SSA_WAVE + to] = u32x2{vr[i][0], vr[i][1]};
-            }
-            wave_lds_sync();
-#pragma unroll
-            for (int i = 0; i < ND; ++i) {
-                if constexpr (KT == 64) {
-                    const u32x4 x = xk[i * SSA_WAVE + from];
-                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][2] = x.z; vr[i][3] = x.w;
-                } else {
-                    const u32x2 x = xv[i * SSA_WAVE + from];
-                    vr[i][0] = x.x; vr[i][1] = x.y;
-                }
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    const PV vf = Ops<T>::value(vr[i][2 * k], vr[i][2 * k + 1], vscale);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int n = NP - 1; n >= 0; --n)
-                            w.o[rt][i] = mfma(vf, pf[rt][k][n], w.o[rt][i]);
-                }
-            }
-            wave_lds_sync();
-        } else {
-            lp2 = look_up(tile + 2 * STEP);
-            pg1 = place(tile + STEP, lp1, entry(lp1));
-            fetch_keys(tile + STEP, pg1);
-        }
-        lp = lp1;
-        pg = pg1;
-        lp1 = lp2;
-    }
-    if constexpr (!SHARED) {
-        w.finish(p, un, un.c0, un.c1, h, split, tile0 < tile1);
-        return;
-    }
-
-    // join the waves: m, l, O in the waves' order
-    if (g == 0)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            m_lds[wave][rt * 16 + col] = w.m[rt];
-            l_lds[wave][rt * 16 + col] = w.l[rt][0];
-        }
-    __syncthreads();                          // (and no wave's pieces are read any more)
-    const float unit = w.unit();
-    for (int v = 0; v < ATT_WAVES; ++v) {
-        if (v == wave) {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                float mx = -INFINITY;
-                for (int i = 0; i < ATT_WAVES; ++i) mx = fmaxf(mx, m_lds[i][rt * 16 + col]);
-                const float a = __builtin_amdgcn_exp2f(w.m[rt] - (mx == -INFINITY ? 0.f : mx)) * unit;
-#pragma unroll
-                for (int i = 0; i < ND; ++i) {
-                    f32x4 *at = (f32x4 *)&o_lds[(rt * 16 + col) * OS + i * 16 + 4 * g];
-                    const f32x4 x = w.o[rt][i] * a;
-                    *at = v == 0 ? x : *at + x;
-                }
-            }
-        }
-        __syncthreads();
-    }
-    for (int i = (int)threadIdx.x; i < CT * D; i += ATT_WAVES * SSA_WAVE) {
-        const int c = i / D, x = i - c * D;
-        if (un.c0 + c >= un.c1) break;
-        float mx = -INFINITY, sum = 0.f;
-        for (int v = 0; v < ATT_WAVES; ++v) mx = fmaxf(mx, m_lds[v][c]);
-        const float ms = mx == -INFINITY ? 0.f : mx;
-        for (int v = 0; v < ATT_WAVES; ++v)
-            sum += l_lds[v][c] * __builtin_amdgcn_exp2f(m_lds[v][c] - ms);
-        const int t = un.t0 + (un.c0 + c) / p.rep, hq = h * p.rep + (un.c0 + c) % p.rep;
-        const float v = o_lds[c * OS + x];
-        if (p.S == 1) {
-            if (x < p.d)
-                Cvt<T>::store((T *)p.out + t * p.o_st + hq * p.o_sh + x,
-                              sum == 0.f ? 0.f : v / sum);
-        } else {
-            const int64_t at = ((int64_t)t * p.Hq + hq) * p.s_stride + split;
-            if (tile0 < tile1) p.part_o[at * D + x] = v;
-            if (x == 0) {
-                p.part_ml[2 * at] = mx;
-                p.part_ml[2 * at + 1] = sum;
-            }
-        }
-    }
+    __shared__ u32x4 lds[attend_lds<D, KT, RT, SHARED>()];
+    attend_unit<T, D, KT, RT, SHARED>(p, blockIdx.x, (int)blockIdx.y, lds);
 }
 
-// Joins the S chunks of each column: one wave per column.  Bound by latency, so the
-// chunks' weights are formed side by side, a lane each.
+// Joins the chunks of each column: D / 4 lanes a column, four channels each.  Bound by
+// latency: the chunks' sums are read four at a time.  In a mixed call `q` describes
+// the prompts' units, numbered behind p's.
 template <typename T, int D>
 __global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE)
-cache_join_kernel(AttendParams p, int CT) {
-    const int lane = lane_id();
-    const int i = (int)blockIdx.x * ATT_WAVES + (int)threadIdx.x / SSA_WAVE;
-    int t, hq;
+cache_join_kernel(AttendParams p, int CT, AttendParams q, int QCT) {
+    constexpr int LC = D / 4, PER = ATT_WAVES * SSA_WAVE / LC;
+    const int x = (int)threadIdx.x % LC * 4;
+    int64_t i = (int64_t)blockIdx.x * PER + (int)threadIdx.x / LC;
+    int t, hq, S = p.S;
     if (p.mode == UNITS_PAGES || p.mode == UNITS_ALL) {    // every row
-        if (i >= p.T * p.Hq) return;
-        t = i / p.Hq;
-        hq = i - t * p.Hq;
+        if (i >= (int64_t)p.T * p.Hq) return;
+        t = (int)i / p.Hq;
+        hq = (int)i - t * p.Hq;
     } else {
+        // whole wavefronts look their unit up together: PER divides CT and QCT
+        const int h = (int)blockIdx.y;
+        const int64_t few = p.S > 1 ? (int64_t)p.units * CT : 0;
         Unit un;
-        const int u = i / CT;
-        if (u >= p.units || !locate_unit(p, u, CT, un)) return;
-        const int c = un.c0 + i - u * CT;
+        int c;
+        if (i < few) {
+            const int u = (int)(i / CT);
+            if (!locate_unit(p, u, CT, un)) return;
+            c = un.c0 + (int)(i - (int64_t)u * CT);
+        } else {
+            i -= few;
+            S = q.S;
+            const int u = (int)(i / QCT);
+            if (S == 1 || u >= q.units || !locate_unit(q, u, QCT, un)) return;
+            c = un.c0 + (int)(i - (int64_t)u * QCT);
+        }
         if (c >= un.c1) return;
         t = un.t0 + c / p.rep;
-        hq = (int)blockIdx.y * p.rep + c % p.rep;
+        hq = h * p.rep + c % p.rep;
     }
     const int64_t row = ((int64_t)t * p.Hq + hq) * p.s_stride;
+    const float2 *ml = (const float2 *)p.part_ml + row;
+    const float *po = p.part_o + row * D + x;
     float mx = -INFINITY;
-    for (int s = lane; s < p.S; s += SSA_WAVE) mx = fmaxf(mx, p.part_ml[2 * (row + s)]);
-    mx = wave_max(mx);
+    for (int s = 0; s < S; ++s) mx = fmaxf(mx, ml[s].x);
     const float ms = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f, o[D / 64];
+    float sum = 0.f;
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < S; s0 += 4) {
+        float w[4];
+        f32x4 v[4];
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) o[j] = 0.f;
-    for (int s0 = 0; s0 < p.S; s0 += SSA_WAVE) {
-        const int s = s0 + lane;
-        float w = 0.f, l = 0.f;
-        if (s < p.S) {
-            l = p.part_ml[2 * (row + s) + 1];
-            w = __builtin_amdgcn_exp2f(p.part_ml[2 * (row + s)] - ms);
+        for (int j = 0; j < 4; ++j) {
+            const int s = min(s0 + j, S - 1);
+            const float2 e = ml[s];
+            // a chunk that saw nothing (l = 0) has written no sums; a NaN is not skipped
+            const bool none = s0 + j >= S || e.y == 0.f;
+            w[j] = none ? 0.f : __builtin_amdgcn_exp2f(e.x - ms);
+            sum += none ? 0.f : e.y * w[j];
+            v[j] = none ? f32x4{0.f, 0.f, 0.f, 0.f} : *(const f32x4 *)(po + (int64_t)s * D);
         }
-        sum += l * w;
-        // a chunk that saw nothing (l = 0) has written no sums; a NaN is not skipped
-        uint64_t some = wave_ballot(l != 0.f);
-        while (some) {
-            const int i = __ffsll((unsigned long long)some) - 1;
-            some &= some - 1;
-            const float wi = __shfl(w, i, SSA_WAVE);
 #pragma unroll
-            for (int j = 0; j < D / 64; ++j)
-                o[j] += p.part_o[(row + s0 + i) * D + j * 64 + lane] * wi;
-        }
+        for (int j = 0; j < 4; ++j) o += v[j] * w[j];
     }
-    sum = wave_sum(sum);
+    T *out = (T *)p.out + t * p.o_st + hq * p.o_sh + x;
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-        const int x = j * 64 + lane;
-        if (x < p.d)
-            Cvt<T>::store((T *)p.out + t * p.o_st + hq * p.o_sh + x, sum == 0.f ? 0.f : o[j] / sum);
-    }
+    for (int j = 0; j < 4; ++j)
+        if (x + j < p.d) Cvt<T>::store(out + j, sum == 0.f ? 0.f : o[j] / sum);
 }
 
 // What a call launches.  A request with more than MANY columns (rows times query
@@ -344,7 +141,8 @@ AttendShape attend_shape(const ssa_cached_attention_args *a) {
         s.units = T * rep / CT + R + 1;
     } else {
         s.mode = UNITS_FEW;
-        s.units = (R + 1) * ceil_div(MANY, CT);
+        s.RT = 1;
+        s.units = (R + 1) * (MANY / 16);
         s.prompt = true;
         // columns per wave: as many as leave two workgroups for every CU
         s.prompt_RT = ssa_cache_prompt_max_rt(a->dtype, c.D);
@@ -383,35 +181,31 @@ int check_attend(const ssa_cached_attention_args *a) {
     return SSA_OK;
 }
 
-template <typename T, int D>
-void launch_join(AttendParams p, int CT, hipStream_t st) {
-    if (p.S == 1) return;
-    const bool all = p.mode == UNITS_PAGES || p.mode == UNITS_ALL;
-    const int64_t columns = all ? (int64_t)p.T * p.Hq : (int64_t)p.units * CT;
-    const dim3 grid((unsigned)ceil_div(columns, ATT_WAVES), all ? 1u : (unsigned)p.Hkv);
-    cache_join_kernel<T, D><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p, CT);
-}
-
 template <typename T, int D, int KT, int RT>
 void launch_attend(const AttendParams &p, const AttendShape &s, hipStream_t st) {
-    if (s.shared) {
+    AttendParams q = p;
+    if (s.prompt) {
+        q.mode = UNITS_MANY;
+        q.units = (int32_t)s.prompt_units;
+        q.S = s.prompt_S;
+        q.chunk = s.prompt_chunk;
+        ssa_cache_mixed_launch(p, q, sizeof(T) == 4 ? SSA_F32 : (__is_same(T, f16_t) ? SSA_F16 : SSA_BF16), D, KT,
+                               s.prompt_RT, st);
+    } else if (s.shared) {
         const dim3 grid((unsigned)(p.units * p.Hkv), (unsigned)p.S);
         cache_attend_kernel<T, D, KT, RT, true><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
     } else {
         const unsigned grid = (unsigned)(ceil_div(p.units, ATT_WAVES) * p.Hkv);
         cache_attend_kernel<T, D, KT, RT, false><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
     }
-    launch_join<T, D>(p, 16 * RT, st);
-    if (s.prompt) {
-        AttendParams pp = p;
-        pp.mode = UNITS_MANY;
-        pp.units = (int32_t)s.prompt_units;
-        pp.S = s.prompt_S;
-        pp.chunk = s.prompt_chunk;
-        ssa_cache_prompt_launch(pp, sizeof(T) == 4 ? SSA_F32 : (__is_same(T, f16_t) ? SSA_F16 : SSA_BF16),
-                                D, KT, s.prompt_RT, st);
-        launch_join<T, D>(pp, ATT_WAVES * 16 * s.prompt_RT, st);
-    }
+    if (p.S == 1 && (!s.prompt || q.S == 1)) return;
+    constexpr int PER = ATT_WAVES * SSA_WAVE / (D / 4);
+    const int QCT = ATT_WAVES * 16 * s.prompt_RT;
+    const int64_t columns = !s.prompt ? (int64_t)p.T * p.Hq
+                                      : (p.S > 1 ? (int64_t)p.units * 16 * RT : 0) +
+                                            (q.S > 1 ? (int64_t)q.units * QCT : 0);
+    const dim3 grid((unsigned)ceil_div(columns, PER), s.prompt ? (unsigned)p.Hkv : 1u);
+    cache_join_kernel<T, D><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p, 16 * RT, q, QCT);
 }
 
 template <typename T, int D>
@@ -457,8 +251,8 @@ extern "C" int ssa_cached_attention(const ssa_cached_attention_args *a, void *wo
     }
     SSA_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "cached_attention: workspace alignment");
     const AttendShape s = attend_shape(a);
-    SSA_CHECK_ARG(s.units * a->cache.Hkv < (1ll << 31) && s.S <= 65535 &&
-                      s.prompt_units * a->cache.Hkv < (1ll << 31) && s.prompt_S <= 65535,
+    SSA_CHECK_ARG((s.units * s.S + s.prompt_units * s.prompt_S) * a->cache.Hkv < (1ll << 31) &&
+                      s.S <= 65535,
                   "cached_attention: too many rows");
     const ssa_kv_cache &c = a->cache;
     AttendParams p = {};

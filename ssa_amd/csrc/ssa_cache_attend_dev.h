@@ -371,6 +371,234 @@ struct Columns {
     }
 };
 
-// launches of ssa_cache_prompt.hip: requests with more columns than `many`
-int ssa_cache_prompt_max_rt(int dtype, int D);          // most 16-column tiles a wave takes
-void ssa_cache_prompt_launch(const AttendParams &p, int dtype, int D, int KT, int RT, hipStream_t st);
+// A unit is 16 RT columns.  SHARED: a workgroup takes one unit and a chunk of its key
+// tiles, its waves every fourth tile, and their sums are joined in LDS.  Otherwise
+// each wave takes a unit of its own and all of its tiles: no joining, for calls with
+// units enough to fill the chip.  A wave holds one tile's values and the next one's
+// keys in flight, and looks page ids up a tile ahead of those.
+// 16-byte pieces of LDS it uses
+template <int D, int KT, int RT, bool SHARED>
+constexpr int attend_lds() {
+    const int moving = ATT_WAVES * KT * D / 16, joined = SHARED ? 16 * RT * (D + 4) / 4 : 0;
+    return (moving > joined ? moving : joined) + ATT_WAVES * 16 * RT / 2;
+}
+
+template <typename T, int D, int KT, int RT, bool SHARED>
+__device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned block, int split,
+                                            u32x4 *lds) {
+    typedef Columns<T, D, KT, RT> C;
+    typedef typename C::PV PV;
+    constexpr int NQ = C::NQ, NP = C::NP, NB = C::NB, DP = C::DP, ND = C::ND, KS = C::KS;
+    constexpr int CT = 16 * RT, OS = D + 4;   // OS: row stride of the joined sums
+    // each wave's pieces on their way to other lanes; then the joined sums
+    u32x4 *x_lds = lds;
+    constexpr int XW = KT * D / 16;
+    float *o_lds = (float *)lds;
+    float (*m_lds)[CT] = (float (*)[CT])(lds + attend_lds<D, KT, RT, SHARED>() - ATT_WAVES * CT / 2);
+    float (*l_lds)[CT] = m_lds + ATT_WAVES;
+
+    const int lane = lane_id(), col = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / SSA_WAVE);
+    // kv heads run fastest: an XCD's workgroups share their heads' pages in its L2
+    const int h = (int)(block % (unsigned)p.Hkv);
+    int u = (int)(block / (unsigned)p.Hkv);
+    if (!SHARED) u = u * ATT_WAVES + wave;
+    Unit un;
+    if (u >= p.units || !locate_unit(p, u, CT, un)) return;
+    C w;
+    w.start(p, un, un.c0, un.c1, h);
+
+    const int page = 1 << p.page_shift, sub_shift = p.page_shift - (KT == 64 ? 6 : 5);
+    const int32_t *list = p.pages ? p.pages + ((int64_t)un.t0 * p.Hkv + h) * p.top : nullptr;
+    const int32_t *table = p.table + (int64_t)(un.req < 0 ? 0 : un.req) * p.table_stride;
+    const int n_tiles = w.most < 0 ? 0 : (list ? p.top << sub_shift : w.most / KT + 1);
+    const int tile0 = split * p.chunk, tile1 = min(tile0 + p.chunk, n_tiles);
+    constexpr int STEP = SHARED ? ATT_WAVES : 1;
+
+    // The logical page of a tile and its entry in the table, looked up a tile ahead
+    // of its keys: the loads are unconditional (of some entry that is there) and
+    // what they say is judged only where it is needed, so nothing waits for them.
+    const int last_entry = (max(tile1, 1) - 1) >> sub_shift;
+    auto look_up = [&](int tile) { return list ? list[min(tile >> sub_shift, last_entry)] : tile >> sub_shift; };
+    auto entry = [&](int lp) { return table[max(0, min(lp, p.width - 1))]; };
+    // the page's place in the cache, -1 if it is absent or unseen
+    auto place = [&](int tile, int lp, int pg) {
+        const int key0 = (lp << p.page_shift) + (tile & ((1 << sub_shift) - 1)) * KT;
+        return tile < tile1 && lp >= 0 && lp < p.width && key0 <= w.most && pg >= 0 && pg < p.num_pages
+                   ? pg : -1;
+    };
+    u32x4 *xk = x_lds + wave * XW;            // [block][64 columns][slot]
+    u32x2 *xv = (u32x2 *)xk;                  // pages of 32: [16 columns][slot]
+    const int lrow = lane >> 2, lpiece = lane & 3, to = slot_of(lrow, lpiece), from = slot_of(col, g);
+    u32x4 kr[NB][DP];
+    float ks = 0.f, vs = 0.f;
+    auto fetch_keys = [&](int tile, int pg) {
+        if (pg < 0) return;
+        const int64_t ph = (int64_t)pg * p.Hkv + h;
+        ks = p.ks[ph];
+        vs = p.vs[ph];
+        const uint8_t *kb = p.k + ph * page * D + (int64_t)(tile & ((1 << sub_shift) - 1)) * KT * D;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < DP; ++i)
+                kr[b][i] = *(const u32x4 *)(kb + (KT / 4 * (lrow >> 2) + 4 * b + (lrow & 3)) * D + i * 64 + lpiece * 16);
+    };
+
+    int tile = tile0 + (SHARED ? wave : 0);
+    int lp = 0, lp1 = 0, pg = -1;
+    if (tile < tile1) {
+        lp = look_up(tile);
+        lp1 = look_up(tile + STEP);
+        pg = place(tile, lp, entry(lp));
+        fetch_keys(tile, pg);
+    }
+    for (; tile < tile1; tile += STEP) {
+        int pg1, lp2;
+        if (pg >= 0) {
+            const int sub = tile & ((1 << sub_shift) - 1);
+            const float kscale = ks, vscale = vs;
+            const uint8_t *vb = p.v + ((int64_t)pg * p.Hkv + h) * D * page + sub * KT;
+            uint32_t vr[ND][KT / 16];
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                const uint8_t *at = vb + ((i * 16 + lrow) << p.page_shift) + KT / 4 * lpiece;
+                if constexpr (KT == 64) {
+                    const u32x4 x = *(const u32x4 *)at;
+                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][2] = x.z; vr[i][3] = x.w;
+                } else {
+                    const u32x2 x = *(const u32x2 *)at;
+                    vr[i][0] = x.x; vr[i][1] = x.y;
+                }
+            }
+            // loads go out in this order: values, then what the next tile's need
+            __builtin_amdgcn_sched_barrier(0);
+            const int entry1 = entry(lp1);
+            lp2 = look_up(tile + 2 * STEP);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < DP; ++i) xk[(b * DP + i) * SSA_WAVE + to] = kr[b][i];
+            wave_lds_sync();
+            f32x4 s[RT][NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) s[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < DP; ++i) {
+                    const u32x4 x = xk[(b * DP + i) * SSA_WAVE + from];
+                    const typename C::QV k0 = Ops<T>::key(x.x, x.y), k1 = Ops<T>::key(x.z, x.w);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int n = NQ - 1; n >= 0; --n) {
+                            s[rt][b] = mfma(k0, w.q[rt][2 * i][n], s[rt][b]);
+                            s[rt][b] = mfma(k1, w.q[rt][2 * i + 1][n], s[rt][b]);
+                        }
+                }
+            }
+            pg1 = place(tile + STEP, lp1, entry1);
+            fetch_keys(tile + STEP, pg1);
+            __builtin_amdgcn_sched_barrier(0);
+            PV pf[RT][KS][NP];
+            w.softmax(s, kscale, vscale, (lp << p.page_shift) + sub * KT, pf);
+            wave_lds_sync();
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                if constexpr (KT == 64)
+                    xk[i * SSA_WAVE + to] = u32x4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]};
+                else
+                    xv[i * SSA_WAVE + to] = u32x2{vr[i][0], vr[i][1]};
+            }
+            wave_lds_sync();
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                if constexpr (KT == 64) {
+                    const u32x4 x = xk[i * SSA_WAVE + from];
+                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][2] = x.z; vr[i][3] = x.w;
+                } else {
+                    const u32x2 x = xv[i * SSA_WAVE + from];
+                    vr[i][0] = x.x; vr[i][1] = x.y;
+                }
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    const PV vf = Ops<T>::value(vr[i][2 * k], vr[i][2 * k + 1], vscale);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int n = NP - 1; n >= 0; --n)
+                            w.o[rt][i] = mfma(vf, pf[rt][k][n], w.o[rt][i]);
+                }
+            }
+            wave_lds_sync();
+        } else {
+            lp2 = look_up(tile + 2 * STEP);
+            pg1 = place(tile + STEP, lp1, entry(lp1));
+            fetch_keys(tile + STEP, pg1);
+        }
+        lp = lp1;
+        pg = pg1;
+        lp1 = lp2;
+    }
+    if constexpr (!SHARED) {
+        w.finish(p, un, un.c0, un.c1, h, split, tile0 < tile1);
+        return;
+    }
+
+    // join the waves: m, l, O in the waves' order
+    if (g == 0)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            m_lds[wave][rt * 16 + col] = w.m[rt];
+            l_lds[wave][rt * 16 + col] = w.l[rt][0];
+        }
+    __syncthreads();                          // (and no wave's pieces are read any more)
+    const float unit = w.unit();
+    for (int v = 0; v < ATT_WAVES; ++v) {
+        if (v == wave) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                float mx = -INFINITY;
+                for (int i = 0; i < ATT_WAVES; ++i) mx = fmaxf(mx, m_lds[i][rt * 16 + col]);
+                const float a = __builtin_amdgcn_exp2f(w.m[rt] - (mx == -INFINITY ? 0.f : mx)) * unit;
+#pragma unroll
+                for (int i = 0; i < ND; ++i) {
+                    f32x4 *at = (f32x4 *)&o_lds[(rt * 16 + col) * OS + i * 16 + 4 * g];
+                    const f32x4 x = w.o[rt][i] * a;
+                    *at = v == 0 ? x : *at + x;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = (int)threadIdx.x; i < CT * D; i += ATT_WAVES * SSA_WAVE) {
+        const int c = i / D, x = i - c * D;
+        if (un.c0 + c >= un.c1) break;
+        float mx = -INFINITY, sum = 0.f;
+        for (int v = 0; v < ATT_WAVES; ++v) mx = fmaxf(mx, m_lds[v][c]);
+        const float ms = mx == -INFINITY ? 0.f : mx;
+        for (int v = 0; v < ATT_WAVES; ++v)
+            sum += l_lds[v][c] * __builtin_amdgcn_exp2f(m_lds[v][c] - ms);
+        const int t = un.t0 + (un.c0 + c) / p.rep, hq = h * p.rep + (un.c0 + c) % p.rep;
+        const float v = o_lds[c * OS + x];
+        if (p.S == 1) {
+            if (x < p.d)
+                Cvt<T>::store((T *)p.out + t * p.o_st + hq * p.o_sh + x,
+                              sum == 0.f ? 0.f : v / sum);
+        } else {
+            const int64_t at = ((int64_t)t * p.Hq + hq) * p.s_stride + split;
+            if (tile0 < tile1) p.part_o[at * D + x] = v;
+            if (x == 0) {
+                p.part_ml[2 * at] = mx;
+                p.part_ml[2 * at + 1] = sum;
+            }
+        }
+    }
+}
+
+// Kernels of ssa_cache_prompt.hip: p's units (requests with at most p.many columns)
+// and q's (the others), side by side; RT 16-column tiles for each of q's waves.
+int ssa_cache_prompt_max_rt(int dtype, int D);
+void ssa_cache_mixed_launch(const AttendParams &p, const AttendParams &q, int dtype, int D, int KT,
+                            int RT, hipStream_t st);

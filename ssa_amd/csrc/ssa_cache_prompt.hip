@@ -12,9 +12,13 @@
 
 namespace {
 
+// 16-byte pieces of LDS a workgroup uses
+template <int D, int KT> constexpr int prompt_lds() {
+    return 2 * 2 * (KT / 16 * (D / 64) + D / 16 * (KT / 32) / 2) * SSA_WAVE + 1;
+}
+
 template <typename T, int D, int KT, int RT>
-__global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE, D <= 128 ? 2 : 1)
-cache_prompt_kernel(AttendParams p) {
+__device__ __forceinline__ void prompt_unit(const AttendParams &p, unsigned block, int split, u32x4 *lds) {
     typedef Columns<T, D, KT, RT> C;
     typedef typename C::QV QV;
     typedef typename C::PV PV;
@@ -22,16 +26,16 @@ cache_prompt_kernel(AttendParams p) {
     constexpr int CT = ATT_WAVES * 16 * RT;
     // a load unit: 16 codes a lane, two fragments
     constexpr int KU = NB * DP, VU = ND * KS / 2, NU = KU + VU, UW = NU / ATT_WAVES;
-    __shared__ u32x4 frag[2][2 * NU][SSA_WAVE];
-    __shared__ int most_lds[ATT_WAVES];
+    u32x4 (*frag)[2 * NU][SSA_WAVE] = (u32x4 (*)[2 * NU][SSA_WAVE])lds;    // two buffers
+    int *most_lds = (int *)(lds + prompt_lds<D, KT>() - 1);
 
     const int lane = lane_id(), lrow = lane >> 2, lpiece = lane & 3;
     const int to = slot_of(lrow, lpiece), from = slot_of(lane & 15, lane >> 4);
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / SSA_WAVE);
     // kv heads run fastest: an XCD's workgroups share their heads' pages in its L2;
     // units run backwards, those with the most keys first
-    const int h = (int)(blockIdx.x % (unsigned)p.Hkv);
-    const int u = p.units - 1 - (int)(blockIdx.x / (unsigned)p.Hkv), split = (int)blockIdx.y;
+    const int h = (int)(block % (unsigned)p.Hkv);
+    const int u = p.units - 1 - (int)(block / (unsigned)p.Hkv);
     Unit un;
     if (!locate_unit(p, u, CT, un)) return;
     const int wc0 = un.c0 + wave * 16 * RT;   // this wave's first column
@@ -162,6 +166,22 @@ cache_prompt_kernel(AttendParams p) {
     w.finish(p, un, wc0, un.c1, h, split, tile0 < tile1);
 }
 
+// Both kinds of units in one launch: requests with few columns (p, first) and with
+// many (q); their lengths, and so which there are, are known on the GPU alone.
+template <typename T, int D, int KT, int RT>
+__global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE, D <= 128 ? 2 : 1)
+cache_mixed_kernel(AttendParams p, AttendParams q) {
+    constexpr int A = attend_lds<D, KT, 1, true>(), B = prompt_lds<D, KT>();
+    __shared__ u32x4 lds[A > B ? A : B];
+    const unsigned pu = (unsigned)(p.units * p.Hkv), few = pu * (unsigned)p.S;
+    if (blockIdx.x < few) {
+        attend_unit<T, D, KT, 1, true>(p, blockIdx.x % pu, (int)(blockIdx.x / pu), lds);
+    } else {
+        const unsigned b = blockIdx.x - few, qu = (unsigned)(q.units * q.Hkv);
+        prompt_unit<T, D, KT, RT>(q, b % qu, (int)(b / qu), lds);
+    }
+}
+
 // Most 16-column tiles of a wave: as many as the registers hold beside O (RT D / 4),
 // the scores and the queries.
 template <typename T, int D> constexpr int max_rt() {
@@ -169,27 +189,27 @@ template <typename T, int D> constexpr int max_rt() {
 }
 
 template <typename T, int D, int RT>
-void launch_rt(const AttendParams &p, int KT, hipStream_t st) {
-    const dim3 grid((unsigned)(p.units * p.Hkv), (unsigned)p.S);
-    if (KT == 32) cache_prompt_kernel<T, D, 32, RT><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
-    else cache_prompt_kernel<T, D, 64, RT><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
+void launch_rt(const AttendParams &p, const AttendParams &q, int KT, hipStream_t st) {
+    const unsigned grid = (unsigned)(p.units * p.Hkv * p.S + q.units * q.Hkv * q.S);
+    if (KT == 32) cache_mixed_kernel<T, D, 32, RT><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p, q);
+    else cache_mixed_kernel<T, D, 64, RT><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p, q);
 }
 
 template <typename T, int D>
-void launch_d(const AttendParams &p, int KT, int RT, hipStream_t st) {
+void launch_d(const AttendParams &p, const AttendParams &q, int KT, int RT, hipStream_t st) {
     constexpr int M = max_rt<T, D>();
     if constexpr (M >= 4)
-        if (RT == 4) return launch_rt<T, D, 4>(p, KT, st);
+        if (RT == 4) return launch_rt<T, D, 4>(p, q, KT, st);
     if constexpr (M >= 2)
-        if (RT == 2) return launch_rt<T, D, 2>(p, KT, st);
-    launch_rt<T, D, 1>(p, KT, st);
+        if (RT == 2) return launch_rt<T, D, 2>(p, q, KT, st);
+    launch_rt<T, D, 1>(p, q, KT, st);
 }
 
 template <typename T>
-void launch_t(const AttendParams &p, int D, int KT, int RT, hipStream_t st) {
-    if (D == 64) launch_d<T, 64>(p, KT, RT, st);
-    else if (D == 128) launch_d<T, 128>(p, KT, RT, st);
-    else launch_d<T, 256>(p, KT, RT, st);
+void launch_t(const AttendParams &p, const AttendParams &q, int D, int KT, int RT, hipStream_t st) {
+    if (D == 64) launch_d<T, 64>(p, q, KT, RT, st);
+    else if (D == 128) launch_d<T, 128>(p, q, KT, RT, st);
+    else launch_d<T, 256>(p, q, KT, RT, st);
 }
 
 }  // namespace
@@ -200,9 +220,9 @@ int ssa_cache_prompt_max_rt(int dtype, int D) {
     return D == 64 ? max_rt<bf16_t, 64>() : (D == 128 ? max_rt<bf16_t, 128>() : max_rt<bf16_t, 256>());
 }
 
-void ssa_cache_prompt_launch(const AttendParams &p, int dtype, int D, int KT, int RT,
-                             hipStream_t st) {
-    if (dtype == SSA_F32) launch_t<float>(p, D, KT, RT, st);
-    else if (dtype == SSA_BF16) launch_t<bf16_t>(p, D, KT, RT, st);
-    else launch_t<f16_t>(p, D, KT, RT, st);
+void ssa_cache_mixed_launch(const AttendParams &p, const AttendParams &q, int dtype, int D, int KT,
+                            int RT, hipStream_t st) {
+    if (dtype == SSA_F32) launch_t<float>(p, q, D, KT, RT, st);
+    else if (dtype == SSA_BF16) launch_t<bf16_t>(p, q, D, KT, RT, st);
+    else launch_t<f16_t>(p, q, D, KT, RT, st);
 }
