@@ -64,27 +64,36 @@ cache_join_kernel(AttendParams p, int CT, AttendParams q, int QCT) {
     const int64_t row = ((int64_t)t * p.Hq + hq) * p.s_stride;
     const float2 *ml = (const float2 *)p.part_ml + row;
     const float *po = p.part_o + row * D + x;
+    // the chunks' maxima and sums, a lane each, LC at a time
+    const int lane = (int)threadIdx.x % LC;
     float mx = -INFINITY;
-    for (int s = 0; s < S; ++s) mx = fmaxf(mx, ml[s].x);
+    for (int s = lane; s < S; s += LC) mx = fmaxf(mx, ml[s].x);
+#pragma unroll
+    for (int k = LC / 2; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k, LC));
     const float ms = mx == -INFINITY ? 0.f : mx;
     float sum = 0.f;
     f32x4 o{0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < S; s0 += 4) {
-        float w[4];
-        f32x4 v[4];
+    for (int b = 0; b < S; b += LC) {
+        const float2 e = b + lane < S ? ml[b + lane] : float2{-INFINITY, 0.f};
+        // a chunk that saw nothing (l = 0) has written no sums; a NaN is not skipped
+        const float w = e.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(e.x - ms);
+        sum += e.y == 0.f ? 0.f : e.y * w;
+        const int n = min(LC, S - b);
+        for (int s0 = 0; s0 < n; s0 += 4) {
+            float wj[4];
+            f32x4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int s = min(s0 + j, S - 1);
-            const float2 e = ml[s];
-            // a chunk that saw nothing (l = 0) has written no sums; a NaN is not skipped
-            const bool none = s0 + j >= S || e.y == 0.f;
-            w[j] = none ? 0.f : __builtin_amdgcn_exp2f(e.x - ms);
-            sum += none ? 0.f : e.y * w[j];
-            v[j] = none ? f32x4{0.f, 0.f, 0.f, 0.f} : *(const f32x4 *)(po + (int64_t)s * D);
+            for (int j = 0; j < 4; ++j) {
+                wj[j] = s0 + j < n ? __shfl(w, s0 + j, LC) : 0.f;
+                v[j] = wj[j] == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f}
+                                    : *(const f32x4 *)(po + (int64_t)(b + s0 + j) * D);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o += v[j] * wj[j];
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o += v[j] * w[j];
     }
+#pragma unroll
+    for (int k = LC / 2; k > 0; k >>= 1) sum += __shfl_xor(sum, k, LC);
     T *out = (T *)p.out + t * p.o_st + hq * p.o_sh + x;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -152,8 +161,11 @@ AttendShape attend_shape(const ssa_cached_attention_args *a) {
         }
         split_tiles(tiles, s.prompt_units * c.Hkv, 512, 4, &s.prompt_S, &s.prompt_chunk);
     }
-    // two tiles or more for each wave
-    split_tiles(tiles, s.units * c.Hkv, 2048, 2 * ATT_WAVES, &s.S, &s.chunk);
+    // Chunks of two tiles or more for each wave.  Lists of pages are equally long: as
+    // many workgroups as the chip holds at once (512: 32 rows of 32 pages 34.7 us, with
+    // 2,048 39.2 us).  Lengths are not: smaller chunks even them out (2,048: 16 tokens
+    // over up to 32k keys 124 us, with 512 128 us, with 4,096 131 us).
+    split_tiles(tiles, s.units * c.Hkv, a->pages ? 512 : 2048, 2 * ATT_WAVES, &s.S, &s.chunk);
     if (!s.prompt && s.units * c.Hkv >= 4096) {
         s.shared = false;
         s.S = 1;

@@ -480,6 +480,11 @@ __device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned bloc
 #pragma unroll
                 for (int i = 0; i < DP; ++i) xk[(b * DP + i) * SSA_WAVE + to] = kr[b][i];
             wave_lds_sync();
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < DP; ++i) kr[b][i] = xk[(b * DP + i) * SSA_WAVE + from];
+            __builtin_amdgcn_sched_barrier(0);
             f32x4 s[RT][NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -487,7 +492,7 @@ __device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned bloc
                 for (int rt = 0; rt < RT; ++rt) s[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < DP; ++i) {
-                    const u32x4 x = xk[(b * DP + i) * SSA_WAVE + from];
+                    const u32x4 x = kr[b][i];
                     const typename C::QV k0 = Ops<T>::key(x.x, x.y), k1 = Ops<T>::key(x.z, x.w);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
@@ -521,6 +526,10 @@ __device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned bloc
                     const u32x2 x = xv[i * SSA_WAVE + from];
                     vr[i][0] = x.x; vr[i][1] = x.y;
                 }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
                     const PV vf = Ops<T>::value(vr[i][2 * k], vr[i][2 * k + 1], vscale);

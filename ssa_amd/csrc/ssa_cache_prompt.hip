@@ -70,15 +70,13 @@ __device__ __forceinline__ void prompt_unit(const AttendParams &p, unsigned bloc
         }
     }
     struct Tile { int pg; float ks, vs; };
-    // the page of a tile, -1 if it is absent
-    auto page_of = [&](int tile) {
-        if (tile >= tile1) return -1;
-        const int pg = table[tile >> sub_shift];
-        return pg >= 0 && pg < p.num_pages ? pg : -1;
-    };
+    // A tile's table entry is loaded a tile ahead of its codes, whatever it is (of the
+    // last tile, past the end), and judged where they are: nothing waits for it.
+    const int last_entry = (max(tile1, 1) - 1) >> sub_shift;
+    auto entry = [&](int tile) { return table[min(tile >> sub_shift, last_entry)]; };
     auto fetch = [&](int tile, int pg, Tile &ti) {
-        ti.pg = pg;
-        if (pg < 0) return;
+        ti.pg = tile < tile1 && pg >= 0 && pg < p.num_pages ? pg : -1;
+        if (ti.pg < 0) return;
         const int sub = tile & ((1 << sub_shift) - 1);
         const int64_t ph = (int64_t)pg * p.Hkv + h;
         ti.ks = p.ks[ph];
@@ -116,10 +114,11 @@ __device__ __forceinline__ void prompt_unit(const AttendParams &p, unsigned bloc
     Tile cur{-1, 0.f, 0.f}, nxt{-1, 0.f, 0.f};
     int pg2 = -1;
     if (tile0 < tile1) {
-        fetch(tile0, page_of(tile0), cur);
+        const int pg0 = entry(tile0), pg1 = entry(tile0 + 1);
+        pg2 = entry(tile0 + 2);
+        fetch(tile0, pg0, cur);
         stage(0, cur);
-        fetch(tile0 + 1, page_of(tile0 + 1), nxt);
-        pg2 = page_of(tile0 + 2);
+        fetch(tile0 + 1, pg1, nxt);
     }
     __syncthreads();
     for (int tile = tile0; tile < tile1; ++tile) {
@@ -127,7 +126,7 @@ __device__ __forceinline__ void prompt_unit(const AttendParams &p, unsigned bloc
         stage(buf ^ 1, nxt);
         Tile nn{-1, 0.f, 0.f};
         fetch(tile + 2, pg2, nn);
-        pg2 = page_of(tile + 3);
+        pg2 = entry(tile + 3);
         const int key0 = tile * KT;
         if (cur.pg >= 0 && key0 <= w.most) {
             f32x4 s[RT][NB];
@@ -135,29 +134,51 @@ __device__ __forceinline__ void prompt_unit(const AttendParams &p, unsigned bloc
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int b = 0; b < NB; ++b) s[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+            // fragments are read a group ahead of the products that take them, the
+            // first values' during the softmax
+            constexpr int KG = DP * 2, VG = ND > 2 ? 2 : ND;
+            const u32x4 *kl = &frag[buf][0][from], *vl = &frag[buf][2 * KU][from];
+            u32x4 kf[2][KG], vf[2][VG * KS];
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int k = 0; k < KG; ++k) kf[0][k] = kl[k * SSA_WAVE];
 #pragma unroll
-                for (int k = 0; k < DP * 2; ++k) {
-                    const QV kf = *(const QV *)&frag[buf][b * DP * 2 + k][from];
+            for (int b = 0; b < NB; ++b) {
+                if (b + 1 < NB) {
+#pragma unroll
+                    for (int k = 0; k < KG; ++k) kf[(b + 1) & 1][k] = kl[((b + 1) * KG + k) * SSA_WAVE];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < VG * KS; ++k) vf[0][k] = vl[k * SSA_WAVE];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < KG; ++k)
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                        for (int n = NQ - 1; n >= 0; --n) s[rt][b] = mfma(kf, w.q[rt][k][n], s[rt][b]);
-                }
+                        for (int n = NQ - 1; n >= 0; --n)
+                            s[rt][b] = mfma(__builtin_bit_cast(QV, kf[b & 1][k]), w.q[rt][k][n], s[rt][b]);
+            }
             PV pf[RT][KS][NP];
             w.softmax(s, cur.ks, cur.vs, key0, pf);
 #pragma unroll
-            for (int i = 0; i < ND; ++i)
+            for (int i = 0; i < ND / VG; ++i) {
+                if (i + 1 < ND / VG)
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    const PV vf = *(const PV *)&frag[buf][2 * KU + i * KS + k][from];
+                    for (int k = 0; k < VG * KS; ++k)
+                        vf[(i + 1) & 1][k] = vl[((i + 1) * VG * KS + k) * SSA_WAVE];
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
+                for (int j = 0; j < VG; ++j)
 #pragma unroll
-                        for (int n = NP - 1; n >= 0; --n)
-                            w.o[rt][i] = mfma(vf, pf[rt][k][n], w.o[rt][i]);
-                }
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                            for (int n = NP - 1; n >= 0; --n)
+                                w.o[rt][i * VG + j] = mfma(__builtin_bit_cast(PV, vf[i & 1][j * KS + k]),
+                                                           pf[rt][k][n], w.o[rt][i * VG + j]);
+            }
         }
         __syncthreads();
         cur = nxt;
@@ -185,7 +206,7 @@ cache_mixed_kernel(AttendParams p, AttendParams q) {
 // Most 16-column tiles of a wave: as many as the registers hold beside O (RT D / 4),
 // the scores and the queries.
 template <typename T, int D> constexpr int max_rt() {
-    return sizeof(T) == 4 ? (D <= 64 ? 2 : 1) : (D <= 64 ? 4 : 2);
+    return sizeof(T) == 4 ? (D <= 64 ? 2 : 1) : (D <= 64 ? 4 : (D <= 128 ? 2 : 1));
 }
 
 template <typename T, int D, int RT>
