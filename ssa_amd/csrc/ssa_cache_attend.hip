@@ -31,7 +31,7 @@ cache_attend_kernel(AttendParams p) {
 // the prompts' units, numbered behind p's.
 template <typename T, int D>
 __global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE)
-cache_join_kernel(AttendParams p, int CT, AttendParams q, int QCT) {
+cache_join_kernel(AttendParams p, AttendParams q, int CT) {
     constexpr int LC = D / 4, PER = ATT_WAVES * SSA_WAVE / LC;
     const int x = (int)threadIdx.x % LC * 4;
     int64_t i = (int64_t)blockIdx.x * PER + (int)threadIdx.x / LC;
@@ -41,7 +41,7 @@ cache_join_kernel(AttendParams p, int CT, AttendParams q, int QCT) {
         t = (int)i / p.Hq;
         hq = (int)i - t * p.Hq;
     } else {
-        // whole wavefronts look their unit up together: PER divides CT and QCT
+        // whole wavefronts look their unit up together: a wave's columns divide CT
         const int h = (int)blockIdx.y;
         const int64_t few = p.S > 1 ? (int64_t)p.units * CT : 0;
         Unit un;
@@ -53,9 +53,9 @@ cache_join_kernel(AttendParams p, int CT, AttendParams q, int QCT) {
         } else {
             i -= few;
             S = q.S;
-            const int u = (int)(i / QCT);
-            if (S == 1 || u >= q.units || !locate_unit(q, u, QCT, un)) return;
-            c = un.c0 + (int)(i - (int64_t)u * QCT);
+            const int u = (int)(i / CT);
+            if (S == 1 || u >= q.units || !locate_unit(q, u, CT, un)) return;
+            c = un.c0 + (int)(i - (int64_t)u * CT);
         }
         if (c >= un.c1) return;
         t = un.t0 + c / p.rep;
@@ -100,21 +100,19 @@ cache_join_kernel(AttendParams p, int CT, AttendParams q, int QCT) {
         if (x + j < p.d) Cvt<T>::store(out + j, sum == 0.f ? 0.f : o[j] / sum);
 }
 
-// What a call launches.  A request with more than MANY columns (rows times query
-// heads of a kv head) shares its keys among that many matrix columns, enough for
-// the kernel that stages key tiles in LDS (ssa_cache_prompt.hip); the others are
-// bound by reading keys and go to the kernel above.  The lengths are on the GPU,
-// so the host goes by T / R alone: at most 4 rows a request on average, all go
-// one way (one launch); else both kernels are launched and each leaves the
-// other's requests.
+// What a call launches.  Many columns (rows times query heads of a kv head) of one
+// request share its keys, staged in LDS (ssa_cache_prompt.hip); single tokens are
+// bound by reading keys and go to the kernel above.  The lengths are on the GPU, so
+// the host goes by T / R alone: at most 4 rows a request on average, all go one way;
+// else all the other, where requests with at most MANY columns are cut into chunks of
+// their keys of their own, having few units each.
 constexpr int MANY = 64;
 
 struct AttendShape {
-    int RT, KT, S, chunk;                     // of the kernel above
-    int mode;
+    int RT, KT, mode, S, chunk;
     int64_t units;
     bool shared, prompt;
-    int prompt_S, prompt_chunk, prompt_RT;
+    int prompt_S, prompt_chunk, columns;      // columns: of a unit
     int64_t prompt_units;
     int s_stride;
 };
@@ -137,28 +135,23 @@ AttendShape attend_shape(const ssa_cached_attention_args *a) {
     s.KT = c.page < 64 ? 32 : 64;
     // two tiles of heads share a wave's keys where the registers hold both
     s.RT = rep > 16 && c.D <= 128 ? 2 : 1;
+    s.columns = 16 * s.RT;
     s.shared = true;
-    const int CT = 16 * s.RT;
     const int per_page = c.page / s.KT;
     int64_t tiles = (int64_t)a->rows.width * per_page;   // the most that a unit can have
     if (a->pages) {
         s.mode = UNITS_PAGES;
-        s.units = T * ceil_div(rep, CT);
+        s.units = T * ceil_div(rep, s.columns);
         tiles = (int64_t)a->top * per_page;
     } else if (T <= 4 * R || T * rep <= MANY) {
         s.mode = UNITS_ALL;
-        s.units = T * rep / CT + R + 1;
+        s.units = T * rep / s.columns + R + 1;
     } else {
         s.mode = UNITS_FEW;
-        s.RT = 1;
-        s.units = (R + 1) * (MANY / 16);
+        s.columns = ssa_cache_prompt_columns(a->dtype, c.D);
+        s.units = (R + 1) * ceil_div(MANY, s.columns);
         s.prompt = true;
-        // columns per wave: as many as leave two workgroups for every CU
-        s.prompt_RT = ssa_cache_prompt_max_rt(a->dtype, c.D);
-        for (;; s.prompt_RT /= 2) {
-            s.prompt_units = T * rep / (ATT_WAVES * 16 * s.prompt_RT) + R + 1;
-            if (s.prompt_RT == 1 || s.prompt_units * c.Hkv >= 512) break;
-        }
+        s.prompt_units = T * rep / s.columns + R + 1;
         split_tiles(tiles, s.prompt_units * c.Hkv, 512, 4, &s.prompt_S, &s.prompt_chunk);
     }
     // Chunks of two tiles or more for each wave.  Lists of pages are equally long: as
@@ -195,41 +188,47 @@ int check_attend(const ssa_cached_attention_args *a) {
 
 template <typename T, int D, int KT, int RT>
 void launch_attend(const AttendParams &p, const AttendShape &s, hipStream_t st) {
-    AttendParams q = p;
-    if (s.prompt) {
-        q.mode = UNITS_MANY;
-        q.units = (int32_t)s.prompt_units;
-        q.S = s.prompt_S;
-        q.chunk = s.prompt_chunk;
-        ssa_cache_mixed_launch(p, q, sizeof(T) == 4 ? SSA_F32 : (__is_same(T, f16_t) ? SSA_F16 : SSA_BF16), D, KT,
-                               s.prompt_RT, st);
-    } else if (s.shared) {
+    if (s.shared) {
         const dim3 grid((unsigned)(p.units * p.Hkv), (unsigned)p.S);
         cache_attend_kernel<T, D, KT, RT, true><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
     } else {
         const unsigned grid = (unsigned)(ceil_div(p.units, ATT_WAVES) * p.Hkv);
         cache_attend_kernel<T, D, KT, RT, false><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
     }
+}
+
+template <typename T, int D>
+void launch_join(const AttendParams &p, const AttendParams &q, const AttendShape &s, hipStream_t st) {
     if (p.S == 1 && (!s.prompt || q.S == 1)) return;
     constexpr int PER = ATT_WAVES * SSA_WAVE / (D / 4);
-    const int QCT = ATT_WAVES * 16 * s.prompt_RT;
     const int64_t columns = !s.prompt ? (int64_t)p.T * p.Hq
-                                      : (p.S > 1 ? (int64_t)p.units * 16 * RT : 0) +
-                                            (q.S > 1 ? (int64_t)q.units * QCT : 0);
+                                      : ((p.S > 1 ? (int64_t)p.units : 0) +
+                                         (q.S > 1 ? (int64_t)q.units : 0)) * s.columns;
     const dim3 grid((unsigned)ceil_div(columns, PER), s.prompt ? (unsigned)p.Hkv : 1u);
-    cache_join_kernel<T, D><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p, 16 * RT, q, QCT);
+    cache_join_kernel<T, D><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p, q, s.columns);
 }
 
 template <typename T, int D>
 void launch_attend_d(const AttendParams &p, const AttendShape &s, hipStream_t st) {
+    AttendParams q = p;
+    if (s.prompt) {
+        q.mode = UNITS_MANY;
+        q.units = (int32_t)s.prompt_units;
+        q.S = s.prompt_S;
+        q.chunk = s.prompt_chunk;
+        const int dtype = sizeof(T) == 4 ? SSA_F32 : (__is_same(T, f16_t) ? SSA_F16 : SSA_BF16);
+        ssa_cache_prompt_launch(p, q, dtype, D, s.KT, st);
+        return launch_join<T, D>(p, q, s, st);
+    }
     if constexpr (D <= 128)
         if (s.RT == 2) {
             if (s.KT == 32) launch_attend<T, D, 32, 2>(p, s, st);
             else launch_attend<T, D, 64, 2>(p, s, st);
-            return;
+            return launch_join<T, D>(p, q, s, st);
         }
     if (s.KT == 32) launch_attend<T, D, 32, 1>(p, s, st);
     else launch_attend<T, D, 64, 1>(p, s, st);
+    launch_join<T, D>(p, q, s, st);
 }
 
 template <typename T>

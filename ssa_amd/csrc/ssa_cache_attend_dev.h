@@ -606,8 +606,8 @@ __device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned bloc
     }
 }
 
-// Kernels of ssa_cache_prompt.hip: p's units (requests with at most p.many columns)
-// and q's (the others), side by side; RT 16-column tiles for each of q's waves.
-int ssa_cache_prompt_max_rt(int dtype, int D);
-void ssa_cache_mixed_launch(const AttendParams &p, const AttendParams &q, int dtype, int D, int KT,
-                            int RT, hipStream_t st);
+// The kernel of ssa_cache_prompt.hip: p's units (requests with at most p.many columns)
+// and q's (the others), ssa_cache_prompt_columns to a workgroup.
+int ssa_cache_prompt_columns(int dtype, int D);
+void ssa_cache_prompt_launch(const AttendParams &p, const AttendParams &q, int dtype, int D, int KT,
+                             hipStream_t st);
