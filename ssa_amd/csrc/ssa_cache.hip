@@ -485,7 +485,8 @@ __device__ __forceinline__ uint64_t score_key64(double s) {
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(NT)
 select_pages_kernel(ssa_select_pages_args a) {
-    constexpr int LP = D / 8, NW = NT / SSA_WAVE, PARTS = NT / D;   // LP lanes of 16 codes a page
+    constexpr int LP = D / 8, NW = NT / SSA_WAVE;           // LP lanes of 16 codes a page
+    constexpr int PARTS = NT < D ? 1 : NT / D;
     extern __shared__ uint64_t sel_keys[];
     __shared__ double qsum[PARTS * 2 * D];
     __shared__ uint32_t hist[2][256];
@@ -505,8 +506,8 @@ select_pages_kernel(ssa_select_pages_args a) {
     }
     // the group's sums of the negative parts of q (for the smallest key codes) and
     // of the positive ones (for the largest)
-    {
-        const int x = tid % D, part = tid / D;
+    for (int i = tid; i < PARTS * D; i += NT) {
+        const int x = i % D, part = i / D;
         double p = 0., m = 0.;
         if (x < c.d)
             for (int g = part; g < rep; g += PARTS) {
@@ -518,7 +519,7 @@ select_pages_kernel(ssa_select_pages_args a) {
         qsum[part * 2 * D + x] = m;
         qsum[part * 2 * D + D + x] = p;
     }
-    if (tid < 256) hist[0][tid] = 0;
+    for (int i = tid; i < 256; i += NT) hist[0][i] = 0;
     if (tid == 0) {
         max_hi = 0;
         min_hi = ~0u;
@@ -540,18 +541,24 @@ select_pages_kernel(ssa_select_pages_args a) {
     const int first = min(a.first, n), last = max(n - a.recent, first);
     const int32_t *table = a.rows.block_table + (int64_t)r * a.rows.table_stride;
     uint32_t mx = 0, mn = ~0u;
-    for (int p0 = first + tid / LP * 4; p0 < last; p0 += NT / LP * 4) {
+    constexpr int STEP = NT / LP * 4;
+    int next[4];                              // page ids, loaded an iteration ahead
+#pragma unroll
+    for (int i = 0; i < 4; ++i) next[i] = table[min(first + tid / LP * 4 + i, n - 1)];
+    for (int p0 = first + tid / LP * 4; p0 < last; p0 += STEP) {
         int pg[4];
         uint4 w[4];
         float sc[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pg[i] = p0 + i < last ? table[p0 + i] : -1;
+        for (int i = 0; i < 4; ++i) pg[i] = p0 + i < last ? next[i] : -1;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int64_t ph = (int64_t)(pg[i] >= 0 && pg[i] < c.num_pages ? pg[i] : 0) * c.Hkv + h;
             w[i] = ((const uint4 *)((const uint8_t *)c.bounds + ph * 2 * D))[sub];
             sc[i] = c.k_scale[ph];
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next[i] = table[min(p0 + STEP + i, n - 1)];
         double s[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -559,10 +566,12 @@ select_pages_kernel(ssa_select_pages_args a) {
             s[i] = 0.;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                s[i] = fma((double)code_f32<0>(ws[j]), qr[4 * j], s[i]);
-                s[i] = fma((double)code_f32<1>(ws[j]), qr[4 * j + 1], s[i]);
-                s[i] = fma((double)code_f32<2>(ws[j]), qr[4 * j + 2], s[i]);
-                s[i] = fma((double)code_f32<3>(ws[j]), qr[4 * j + 3], s[i]);
+                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)ws[j], false);
+                const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)ws[j], true);
+                s[i] = fma((double)lo[0], qr[4 * j], s[i]);
+                s[i] = fma((double)lo[1], qr[4 * j + 1], s[i]);
+                s[i] = fma((double)hi[0], qr[4 * j + 2], s[i]);
+                s[i] = fma((double)hi[1], qr[4 * j + 3], s[i]);
             }
             s[i] *= (double)sc[i];
         }
@@ -607,7 +616,7 @@ select_pages_kernel(ssa_select_pages_args a) {
                 if ((k >> bits) == prefix)
                     atomicAdd(&hist[buf][(uint32_t)k & ((1u << bits) - 1u)], 1u);
             }
-            if (tid < 256) hist[buf ^ 1][tid] = 0;
+            for (int i = tid; i < 256; i += NT) hist[buf ^ 1][i] = 0;
             __syncthreads();
             if (wave == 0) {                // four digits a lane, sums from the top
                 uint32_t b[4], own = 0;
@@ -679,11 +688,14 @@ int launch_select(const ssa_select_pages_args &a, hipStream_t s) {
 }
 
 // Few rows: a CU has one workgroup or none, and 16 waves shorten its walk over the
-// pages.  Many: 4 waves, so that several workgroups hide each other's latency.
+// pages.  Many: a wave each, with no barriers to wait at (1,000 rows of 4 heads over 250
+// pages: 29 us with 4 waves), where the LDS holds enough of them.
 template <typename T, int D>
 int launch_select_d(const ssa_select_pages_args &a, hipStream_t s) {
-    return (int64_t)a.rows.T * a.cache.Hkv <= 512 ? launch_select<T, D, 1024>(a, s)
-                                                  : launch_select<T, D, 256>(a, s);
+    const int64_t n = (int64_t)a.rows.T * a.cache.Hkv;
+    if (n <= 512) return launch_select<T, D, 1024>(a, s);
+    return n > 2048 && a.rows.width <= 1024 ? launch_select<T, D, 64>(a, s)
+                                            : launch_select<T, D, 256>(a, s);
 }
 
 template <typename T>

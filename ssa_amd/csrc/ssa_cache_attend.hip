@@ -20,7 +20,7 @@
 namespace {
 
 template <typename T, int D, int KT, int RT, bool SHARED>
-__global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE, D <= 128 && RT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE, D <= 128 && RT == 1 ? (SHARED || sizeof(T) == 4 ? 2 : 3) : 1)
 cache_attend_kernel(AttendParams p) {
     __shared__ u32x4 lds[attend_lds<D, KT, RT, SHARED>()];
     attend_unit<T, D, KT, RT, SHARED>(p, blockIdx.x, (int)blockIdx.y, lds);

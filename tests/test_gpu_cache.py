@@ -469,6 +469,104 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(got, ref.select(q, small, [[0, 1, 2]], [0, 0], [148, 149], 2, 1, 1))
 
 
+# ---------------------------------------------------------------------------- forms
+# Which kernel and how many chunks a call takes follows from T, R, heads, table width and
+# page size; these reach the forms that the small cases above do not.
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("d,ps", [(64, 32), (128, 64), (200, 128)])
+def test_attention_of_many_single_tokens(dtype, d, ps):
+    """Units enough that each wave takes one of its own: 700 requests, 8 kv heads."""
+    g = _gen(d)
+    R = 700
+    lens = torch.randint(1, 3 * ps, (R,), generator=g).tolist()
+    new = [1] * R
+    new[5], new[9] = 0, 3
+    lens[9] += 3
+    b = _batch(lens, new, ps, 3 * R, d, extra=1)
+    c = _random_cache(3 * R, 8, d, ps, d)
+    q, qd = _queries(len(b[2]), 8, d, dtype, 3)
+    _check_attend(c, b, q, qd)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("Hq,H,d,ps", [(8, 8, 64, 32), (32, 8, 128, 64), (40, 2, 96, 128)])
+def test_attention_over_chosen_pages_for_many_rows(dtype, Hq, H, d, ps):
+    """Lists for rows enough to fill the chip, one wave a list."""
+    T = 4096 // H + 40
+    b = _batch([30 * ps + 5, 2 * ps + T], [40, T], ps, 100 + T // ps, d)
+    rows = len(b[2])
+    c = _random_cache(100 + T // ps, H, d, ps, d)
+    g = _gen(d)
+    pages = torch.stack([torch.randperm(12, generator=g)[:3] for _ in range(rows * H)])
+    pages = pages.reshape(rows, H, 3).int()
+    q, qd = _queries(rows, Hq, d, dtype, 4)
+    _check_attend(c, b, q, qd, pages=pages)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("Hq,H,d,ps", [(4, 4, 64, 32), (8, 2, 128, 64), (6, 1, 256, 128)])
+def test_attention_of_a_prompt_behind_a_long_context(dtype, Hq, H, d, ps):
+    """A prompt's keys in several chunks, single tokens with their own beside it, in
+    one call; and pages missing in the middle."""
+    lens = [70 * ps + 11, 33 * ps, 2, 50 * ps + 1]
+    b = _batch(lens, [90, 1, 0, 3], ps, 200, d, extra=2)
+    b[0][0][20] = b[0][3][7] = -1
+    b[0][0][21] = 5000
+    c = _random_cache(200, H, d, ps, d)
+    q, qd = _queries(len(b[2]), Hq, d, dtype, 5, strided=True)
+    got = _check_attend(c, b, q, qd)
+    assert bool((got[-2:] == 0).all())
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 30.0])
+def test_attention_scales(scale):
+    """Negative, zero and large factors: the running maximum is the scaled scores'."""
+    ps, d = 64, 64
+    for new in ([1, 1], [100, 1]):
+        b = _batch([150, 70], new, ps, 9, 1)
+        c = _random_cache(9, 2, d, ps, 1)
+        q, qd = _queries(len(b[2]), 4, d, F32, 6)
+        _check_attend(c, b, q, qd, scale=scale)
+
+
+def test_a_bad_token_in_a_prompt():
+    """NaN and infinite tokens inside a prompt's own rows: causal rows before them and
+    other heads stay finite, in every form."""
+    ps, d, H = 32, 64, 2
+    for dtype in (F32, BF16, F16):
+        c = _random_cache(12, H, d, ps, 2)
+        b = _batch([130, 60], [100, 2], ps, 12, 2)
+        g = _gen(4)
+        for key, bad in ((57, math.nan), (100, math.inf)):
+            k, v = torch.randn(1, H, d, generator=g), torch.randn(1, H, d, generator=g)
+            v[0, 0, 3] = bad
+            s = torch.tensor([b[0][0][key // ps] * ps + key % ps], device=DEV)
+            ssa_amd.cache_append(c, k.to(DEV), v.to(DEV), s)
+        q, qd = _queries(102, 4, d, dtype, 12)
+        got = _check_attend(c, b, q, qd)
+        nan = got.isnan().any(-1).cpu()
+        seen = torch.tensor([r == 0 and p >= 57 for r, p in zip(b[2], b[3])])
+        assert torch.equal(nan[:, :2].all(1), seen) and not bool(nan[:, 2:].any())
+
+
+def test_select_of_many_rows():
+    """Rows enough for a wave each, beside requests without enough pages to choose."""
+    ps, d, H = 32, 64, 4
+    b = _batch([60 * ps + 3, 700, 9], [500, 60, 1], ps, 100, 1, extra=2)
+    c = _random_cache(100, H, d, ps, 1)
+    q, qd = _queries(len(b[2]), 8, d, BF16, 2)
+    got = ssa_amd.select_pages(qd, c, _plan(b), 7, first=2, recent=2)
+    assert torch.equal(got.cpu(), ref.select(q, ref.Cache.of(c), b[0], b[2], b[3], 7, 2, 2))
+
+
+@pytest.mark.parametrize("R", [256, 257, 1024, 1025, 4096, 4097])
+def test_plan_at_the_bounds_of_its_forms(R):
+    g = _gen(R)
+    cached = torch.randint(0, 70, (R,), generator=g).tolist()
+    new = torch.randint(0, 4, (R,), generator=g).tolist()
+    _check_plan(cached, new, 3, torch.randperm(2 * R, generator=g).tolist(), R // 3, 32, 2 * R)
+
+
 # ---------------------------------------------------------------------------- as used
 def _layer(**kw):
     a = dict(d_model=256, num_heads=8, num_kv_heads=2, num_neighbors=128, window_size=16,
