@@ -406,8 +406,10 @@ int ssa_select_pages(const ssa_select_pages_args *a, void *stream);
  * negative: none; each page at most once).  q and out (T, Hq, d), unit last
  * strides; out in q's type.  Query head g reads kv head g / (Hq / Hkv).  Products
  * of q and codes are exact, sums and softmax in fp32, probabilities to 11 bits or
- * more (24 for fp32 q).  A row that sees no key gets zeros.  Needs a 16-byte aligned
- * workspace of ssa_cached_attention_workspace_bytes (0 for some sizes). */
+ * more (24 for fp32 q).  A row that sees no key, or whose every score is -inf, gets
+ * zeros.  For 16-bit q the values of a page more than 2^64 below the largest of the
+ * request and head count as zeros.  starts[0] = 0.  Needs a 16-byte aligned workspace
+ * of ssa_cached_attention_workspace_bytes (0 for some sizes, about 130 MB at most). */
 typedef struct {
     ssa_kv_cache cache;
     ssa_batch_rows rows;

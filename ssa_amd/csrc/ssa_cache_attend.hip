@@ -36,34 +36,37 @@ cache_join_kernel(AttendParams p, AttendParams q, int CT) {
     const int x = (int)threadIdx.x % LC * 4;
     int64_t i = (int64_t)blockIdx.x * PER + (int)threadIdx.x / LC;
     int t, hq, S = p.S;
+    const float *mls = p.part_ml, *pos = p.part_o;
+    int64_t row;
     if (p.mode == UNITS_PAGES || p.mode == UNITS_ALL) {    // every row
         if (i >= (int64_t)p.T * p.Hq) return;
         t = (int)i / p.Hq;
         hq = (int)i - t * p.Hq;
+        row = i * S;
     } else {
         // whole wavefronts look their unit up together: a wave's columns divide CT
         const int h = (int)blockIdx.y;
         const int64_t few = p.S > 1 ? (int64_t)p.units * CT : 0;
-        Unit un;
-        int c;
-        if (i < few) {
-            const int u = (int)(i / CT);
-            if (!locate_unit(p, u, CT, un)) return;
-            c = un.c0 + (int)(i - (int64_t)u * CT);
-        } else {
+        const bool is_few = i < few;
+        if (!is_few) {
             i -= few;
             S = q.S;
-            const int u = (int)(i / CT);
-            if (S == 1 || u >= q.units || !locate_unit(q, u, CT, un)) return;
-            c = un.c0 + (int)(i - (int64_t)u * CT);
+            mls = q.part_ml;
+            pos = q.part_o;
         }
+        const int u = (int)(i / CT);
+        Unit un;
+        if (is_few ? !locate_unit(p, u, CT, un)
+                   : S == 1 || u >= q.units || !locate_unit(q, u, CT, un))
+            return;
+        const int c = un.c0 + (int)(i - (int64_t)u * CT);
         if (c >= un.c1) return;
         t = un.t0 + c / p.rep;
         hq = h * p.rep + c % p.rep;
+        row = part_of(is_few ? p : q, un, c, h);
     }
-    const int64_t row = ((int64_t)t * p.Hq + hq) * p.s_stride;
-    const float2 *ml = (const float2 *)p.part_ml + row;
-    const float *po = p.part_o + row * D + x;
+    const float2 *ml = (const float2 *)mls + row;
+    const float *po = pos + row * D + x;
     // the chunks' maxima and sums, a lane each, LC at a time
     const int lane = (int)threadIdx.x % LC;
     float mx = -INFINITY;
@@ -114,7 +117,7 @@ struct AttendShape {
     bool shared, prompt;
     int prompt_S, prompt_chunk, columns;      // columns: of a unit
     int64_t prompt_units;
-    int s_stride;
+    int64_t parts, prompt_parts;              // columns times chunks in the workspace
 };
 
 // chunks of the key tiles: about `wgs` workgroups in all, `least` tiles or more each
@@ -149,7 +152,7 @@ AttendShape attend_shape(const ssa_cached_attention_args *a) {
     } else {
         s.mode = UNITS_FEW;
         s.columns = ssa_cache_prompt_columns(a->dtype, c.D);
-        s.units = (R + 1) * ceil_div(MANY, s.columns);
+        s.units = R + 1;
         s.prompt = true;
         s.prompt_units = T * rep / s.columns + R + 1;
         split_tiles(tiles, s.prompt_units * c.Hkv, 512, 4, &s.prompt_S, &s.prompt_chunk);
@@ -164,7 +167,10 @@ AttendShape attend_shape(const ssa_cached_attention_args *a) {
         s.S = 1;
         s.chunk = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
     }
-    s.s_stride = s.prompt && s.prompt_S > s.S ? s.prompt_S : s.S;
+    // no chunks, no parts; else about 2,048 workgroups' columns at most
+    const int64_t few = s.prompt ? s.units * c.Hkv * MANY : T * a->Hq;
+    s.parts = s.S > 1 ? few * s.S : 0;
+    s.prompt_parts = s.prompt && s.prompt_S > 1 ? T * a->Hq * s.prompt_S : 0;
     return s;
 }
 
@@ -216,6 +222,8 @@ void launch_attend_d(const AttendParams &p, const AttendShape &s, hipStream_t st
         q.units = (int32_t)s.prompt_units;
         q.S = s.prompt_S;
         q.chunk = s.prompt_chunk;
+        q.part_ml = p.part_o + s.parts * D;
+        q.part_o = q.part_ml + s.prompt_parts * 2;
         const int dtype = sizeof(T) == 4 ? SSA_F32 : (__is_same(T, f16_t) ? SSA_F16 : SSA_BF16);
         ssa_cache_prompt_launch(p, q, dtype, D, s.KT, st);
         return launch_join<T, D>(p, q, s, st);
@@ -245,8 +253,7 @@ extern "C" int64_t ssa_cached_attention_workspace_bytes(const ssa_cached_attenti
     if (rc != SSA_OK) return rc;
     if (a->rows.T == 0) return 0;
     const AttendShape s = attend_shape(a);
-    if (s.s_stride == 1) return 0;
-    return (int64_t)a->rows.T * a->Hq * s.s_stride * (2 + a->cache.D) * 4;
+    return (s.parts + s.prompt_parts) * (2 + a->cache.D) * 4;
 }
 
 extern "C" int ssa_cached_attention(const ssa_cached_attention_args *a, void *workspace,
@@ -279,7 +286,7 @@ extern "C" int ssa_cached_attention(const ssa_cached_attention_args *a, void *wo
     p.q = a->q;
     p.out = a->out;
     p.part_ml = (float *)workspace;
-    p.part_o = p.part_ml + (int64_t)a->rows.T * a->Hq * s.s_stride * 2;
+    p.part_o = p.part_ml + s.parts * 2;
     p.num_pages = c.num_pages;
     p.table_stride = a->rows.table_stride;
     p.q_st = a->q_st;
@@ -296,7 +303,6 @@ extern "C" int ssa_cached_attention(const ssa_cached_attention_args *a, void *wo
     p.page_shift = c.page == 32 ? 5 : (c.page == 64 ? 6 : 7);
     p.top = a->top;
     p.S = s.S;
-    p.s_stride = s.s_stride;
     p.mode = s.mode;
     p.many = MANY;
     p.units = (int32_t)s.units;

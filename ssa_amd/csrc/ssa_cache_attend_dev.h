@@ -19,7 +19,7 @@ constexpr float LOG2E = 1.44269504088896340736f;
 enum {
     UNITS_PAGES,    // unit = row and group of its heads
     UNITS_ALL,      // every request's groups
-    UNITS_FEW,      // those of requests with at most `many` columns, numbered by request
+    UNITS_FEW,      // one for each request with at most `many` columns (CT >= many)
     UNITS_MANY,     // those of the others
 };
 
@@ -29,22 +29,32 @@ struct AttendParams {
     const int32_t *table, *starts, *requests, *positions, *pages;
     const void *q;
     void *out;
-    float *part_ml, *part_o;                  // (T * Hq, s_stride, 2), (T * Hq, s_stride, D)
+    float *part_ml, *part_o;                  // (columns, S, 2), (columns, S, D)
     int64_t num_pages, table_stride, q_st, q_sh, o_st, o_sh;
-    int32_t T, R, width, Hq, Hkv, rep, d, page_shift, top, S, s_stride, chunk, mode, many, units;
+    int32_t T, R, width, Hq, Hkv, rep, d, page_shift, top, S, chunk, mode, many, units;
     int32_t q_vec, o_vec;                     // rows of q in 16-byte pieces, of out in 4 elements
     float scale;                              // softmax scale * log2(e)
 };
 
 struct Unit {
     int req, t0, c0, c1;    // row t0 + c / rep, head c % rep, for c in [c0, c1)
+    int u;
 };
+
+// Where the chunks of a column are: by row and head; in UNITS_FEW, whose requests are
+// cut into more chunks than all rows have room for, by unit and column.
+__device__ __forceinline__ int64_t part_of(const AttendParams &p, const Unit &x, int c, int h) {
+    if (p.mode == UNITS_FEW) return (((int64_t)x.u * p.Hkv + h) * p.many + c) * p.S;
+    const int t = x.t0 + c / p.rep;
+    return ((int64_t)t * p.Hq + h * p.rep + c % p.rep) * p.S;
+}
 
 // The columns of unit u, false if there are none.  Requests' units are numbered
 // without a list: in UNITS_ALL and UNITS_MANY request r (R stands for the rows
 // behind the last one) has its units from floor(starts[r] rep / CT) + r on, which
 // leaves each request ceil(rows rep / CT); found by binary search.
 __device__ __forceinline__ bool locate_unit(const AttendParams &p, int u, int CT, Unit &x) {
+    x.u = u;
     if (p.mode == UNITS_PAGES) {
         const int tiles = (p.rep + CT - 1) / CT;
         x.t0 = u / tiles;
@@ -55,9 +65,8 @@ __device__ __forceinline__ bool locate_unit(const AttendParams &p, int u, int CT
         int lo = 0;
         int64_t j;
         if (p.mode == UNITS_FEW) {
-            const int tiles = (p.many + CT - 1) / CT;
-            lo = u / tiles;
-            j = u - lo * tiles;
+            lo = u;                           // CT >= many: one a request
+            j = 0;
             x.t0 = p.starts[lo];
         } else {
             // last r whose first unit is <= u: the wave tests 64 places of lo .. hi at
@@ -160,13 +169,15 @@ template <> struct Ops<float> {
 // Per score the vector unit does a maximum, a fused multiply-add, an exponential and
 // half a conversion; everything else is kept off that path:
 //  * the key scale of a page goes into the multiply-add's constant, the value scale
-//    2^e_v into its addend: O is kept in units of 2^e_ref and p_j 2^(e_v - e_ref) is
-//    what multiplies the unscaled codes;
+//    2^e_v into its addend: O is kept in units of 2^e_ref and p_j 2^lift, lift = e_v -
+//    e_ref, is what multiplies the unscaled codes;
 //  * sums of p come from the matrix unit, as one more row of V^T (the power of two
 //    that undoes these units, so that they are the sums of p as rounded);
-//  * O is rescaled only when a column's maximum has grown by more than 2^4, or
-//    e_v - e_ref has left 0 .. 6; with 2^5 to spare below, p 2^5 2^(e_v - e_ref) as an
-//    f16 stays under 2^15 and its rounding at 11 bits, or 2^-30 of the largest p.
+//  * O is rescaled only when a column's maximum has grown by more than 2^4, or lift
+//    has left 0 .. 6.  With 2^5 to spare below, p 2^(lift + 5) as an f16 stays under
+//    2^15 and its rounding at 11 bits, or 2^-30 of the largest p.  Values more than
+//    2^64 below the request's largest (of a page of zeros, as a rule, which has the
+//    smallest scale there is) are taken as zeros: O in their units could leave fp32.
 // For fp32 queries p is three bf16 terms (24 bits; V scaled, as bf16 holds every
 // scale).
 template <typename T, int D, int KT, int RT>
@@ -178,11 +189,13 @@ struct Columns {
     static constexpr int NQ = O_::NQ, NP = O_::NP;
     static constexpr int NB = KT / 16, DP = D / 64, ND = D / 16, KS = KT / 32;
     // p is kept 2^ROOM larger, O in units of 2^(e_ref - ROOM)
-    static constexpr float ROOM = F32 ? 0.f : 5.f, GROWN = 4.f, LIFT = 6.f;
+    static constexpr int ROOM = F32 ? 0 : 5, LIFT = 6;
+    static constexpr float GROWN = 4.f;
 
     QV q[RT][DP * 2][NQ];
     f32x4 o[RT][ND], l[RT];
-    float m[RT], e_ref, scale;
+    float m[RT], scale;
+    int e_ref, e_top;            // O's unit; the largest it has been
     int pos[RT];                 // last key a column sees; none for it to lose if it is dead
     int most, least;             // of the live columns
 
@@ -191,7 +204,7 @@ struct Columns {
         const int lane = lane_id(), col = lane & 15, g = lane >> 4;
         const bool neg = p.scale < 0.f;
         scale = fabsf(p.scale);
-        e_ref = 0.f;
+        e_ref = e_top = -10000;  // anything is larger, and O is 0
         most = -1;
         least = 0x7fffffff;
 #pragma unroll
@@ -246,9 +259,9 @@ struct Columns {
     }
 
     // scores to probabilities: key scale ks, value scale vs, first key of the tile;
-    // l takes their sums
-    __device__ __forceinline__ void softmax(f32x4 (&s)[RT][NB], float ks, float vs, int key0,
-                                            PV (&pf)[RT][KS][NP]) {
+    // l takes their sums.  False where the tile's values count as zeros.
+    __device__ __forceinline__ bool softmax(f32x4 (&s)[RT][NB], float ks, float vs, int key0,
+                                             PV (&pf)[RT][KS][NP]) {
         const int g = lane_id() >> 4;
         float c = scale * ks;                 // log2 units of a score's unit
         if (key0 + KT - 1 > least) {          // some column ends in this tile
@@ -262,7 +275,7 @@ struct Columns {
                                                                               : -INFINITY;
             c = 1.f;
         }
-        const float ev = F32 ? 0.f : (float)((int)(__float_as_uint(vs) >> 23) - 127);
+        const int ev = F32 ? 0 : (int)(__builtin_amdgcn_readfirstlane(__float_as_uint(vs)) >> 23) - 127;
         float mx[RT];
         bool grow = false;
 #pragma unroll
@@ -275,10 +288,13 @@ struct Columns {
             mx[rt] = v * c;
             grow |= mx[rt] > m[rt] + GROWN;
         }
-        if (wave_ballot(grow) || ev < e_ref || ev > e_ref + LIFT) {
-            const float e_new = F32 ? 0.f : ev - 3.f;
-            const float unit = __builtin_amdgcn_exp2f(e_ref - e_new);
+        const bool tiny = !F32 && ev < e_top - 64;
+        const bool move = !tiny && (ev > e_ref + LIFT || ev < e_ref);
+        if (wave_ballot(grow) || move) {
+            const int e_new = move ? (F32 ? 0 : ev - 3) : e_ref;
+            const float unit = __builtin_amdgcn_exp2f((float)(e_ref - e_new));
             e_ref = e_new;
+            e_top = max(e_top, e_new);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 float v = mx[rt];
@@ -293,7 +309,7 @@ struct Columns {
                 for (int i = 0; i < ND; ++i) o[rt][i] *= au;
             }
         }
-        const float lift = ev - e_ref + ROOM;
+        const float lift = (float)(tiny ? ROOM : ev - e_ref + ROOM);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const float sub = lift - (m[rt] == -INFINITY ? 0.f : m[rt]);
@@ -320,9 +336,10 @@ struct Columns {
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int n = NP - 1; n >= 0; --n) l[rt] = mfma(ones, pf[rt][k][n], l[rt]);
+        return !tiny;
     }
 
-    __device__ __forceinline__ float unit() const { return __builtin_amdgcn_exp2f(e_ref - ROOM); }
+    __device__ __forceinline__ float unit() const { return __builtin_amdgcn_exp2f((float)(e_ref - ROOM)); }
 
     // results, or this chunk's part of them
     __device__ __forceinline__ void finish(const AttendParams &p, const Unit &u, int c0, int c1, int h,
@@ -356,7 +373,7 @@ struct Columns {
                     }
                 }
             } else {
-                const int64_t at = ((int64_t)t * p.Hq + hq) * p.s_stride + split;
+                const int64_t at = part_of(p, u, c, h) + split;
                 if (any) {
 #pragma unroll
                     for (int i = 0; i < ND; ++i)
@@ -507,38 +524,39 @@ __device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned bloc
             fetch_keys(tile + STEP, pg1);
             __builtin_amdgcn_sched_barrier(0);
             PV pf[RT][KS][NP];
-            w.softmax(s, kscale, vscale, (lp << p.page_shift) + sub * KT, pf);
+            const bool some = w.softmax(s, kscale, vscale, (lp << p.page_shift) + sub * KT, pf);
             wave_lds_sync();
+            if (some) {
 #pragma unroll
-            for (int i = 0; i < ND; ++i) {
-                if constexpr (KT == 64)
-                    xk[i * SSA_WAVE + to] = u32x4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]};
-                else
-                    xv[i * SSA_WAVE + to] = u32x2{vr[i][0], vr[i][1]};
-            }
-            wave_lds_sync();
-#pragma unroll
-            for (int i = 0; i < ND; ++i) {
-                if constexpr (KT == 64) {
-                    const u32x4 x = xk[i * SSA_WAVE + from];
-                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][2] = x.z; vr[i][3] = x.w;
-                } else {
-                    const u32x2 x = xv[i * SSA_WAVE + from];
-                    vr[i][0] = x.x; vr[i][1] = x.y;
+                for (int i = 0; i < ND; ++i) {
+                    if constexpr (KT == 64)
+                        xk[i * SSA_WAVE + to] = u32x4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]};
+                    else
+                        xv[i * SSA_WAVE + to] = u32x2{vr[i][0], vr[i][1]};
                 }
-            }
-            __builtin_amdgcn_sched_barrier(0);
+                wave_lds_sync();
 #pragma unroll
-            for (int i = 0; i < ND; ++i) {
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    const PV vf = Ops<T>::value(vr[i][2 * k], vr[i][2 * k + 1], vscale);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int n = NP - 1; n >= 0; --n)
-                            w.o[rt][i] = mfma(vf, pf[rt][k][n], w.o[rt][i]);
+                for (int i = 0; i < ND; ++i) {
+                    if constexpr (KT == 64) {
+                        const u32x4 x = xk[i * SSA_WAVE + from];
+                        vr[i][0] = x.x; vr[i][1] = x.y; vr[i][2] = x.z; vr[i][3] = x.w;
+                    } else {
+                        const u32x2 x = xv[i * SSA_WAVE + from];
+                        vr[i][0] = x.x; vr[i][1] = x.y;
+                    }
                 }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < ND; ++i)
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const PV vf = Ops<T>::value(vr[i][2 * k], vr[i][2 * k + 1], vscale);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                            for (int n = NP - 1; n >= 0; --n)
+                                w.o[rt][i] = mfma(vf, pf[rt][k][n], w.o[rt][i]);
+                    }
             }
             wave_lds_sync();
         } else {
@@ -596,7 +614,7 @@ __device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned bloc
                 Cvt<T>::store((T *)p.out + t * p.o_st + hq * p.o_sh + x,
                               sum == 0.f ? 0.f : v / sum);
         } else {
-            const int64_t at = ((int64_t)t * p.Hq + hq) * p.s_stride + split;
+            const int64_t at = part_of(p, un, un.c0 + c, h) + split;
             if (tile0 < tile1) p.part_o[at * D + x] = v;
             if (x == 0) {
                 p.part_ml[2 * at] = mx;

@@ -228,10 +228,11 @@ class PageTable:
         return p
 
     def release(self, places: torch.Tensor) -> None:
-        """Give the pages of these places (integer tensor) back and empty them."""
+        """Give the pages of these places (integer tensor; what names no place is
+        passed over) back and empty them."""
         R, W = self.block_table.shape
-        gone = torch.zeros(R, dtype=torch.bool, device=self.lengths.device)
-        gone[places.to(self.lengths.device, torch.int64)] = True
+        places = places.to(self.lengths.device, torch.int64).reshape(1, -1)
+        gone = (torch.arange(R, device=self.lengths.device)[:, None] == places).any(1)
         held = (self.lengths + self.page_size - 1) // self.page_size
         col = torch.arange(W, device=self.lengths.device)
         give = (gone[:, None] & (col < held[:, None])).reshape(-1)

@@ -204,7 +204,9 @@ def attend(q, c, table, requests, positions, scale, pages=None):
 def attend_tolerance(out, spread, reach, size, dtype, keys, d):
     """How far a result may be from `out`, per element.
 
-    The result is rounded to its type once: finfo.eps / 2 of its value.  A
+    The result is rounded to its type once: off by finfo.eps / 2 of its value, or,
+    below the type's normal numbers (f16's reach to 2^-14), by half the step that
+    they all have, tiny * eps.  A
     probability p is rounded to f16 (fp32 queries: to three bf16 terms, 24 bits):
     off by 2^-11 of its value (2^-24), and where that f16 is subnormal by half its
     step, 2^-25: 2^-30 of the largest p, which is kept 2^5 above 1.  The numerator
@@ -215,7 +217,7 @@ def attend_tolerance(out, spread, reach, size, dtype, keys, d):
     step truncates), which enters the exponential, the sum and the maximum: twice.
     The exponential is off by 2^-22; the sums over the keys by keys * 2^-23 each,
     the numerator's and the denominator's."""
-    half = torch.finfo(dtype).eps / 2
+    half, least_step = torch.finfo(dtype).eps / 2, torch.finfo(dtype).tiny * torch.finfo(dtype).eps
     term, least = (2.0 ** -24, 0.0) if dtype == torch.float32 else (2 * 2.0 ** -11, 2.0 ** -29)
     rel = term + 2 * (d + 2) * 2.0 ** -23 * reach + 2.0 ** -21 + 2 * keys * 2.0 ** -23
-    return half * out.abs() + (1 + half) * (rel * spread + least * keys * size) + 2.0 ** -120
+    return half * out.abs() + (1 + half) * (rel * spread + least * keys * size) + least_step / 2 + 2.0 ** -120

@@ -230,6 +230,20 @@ def test_c_entry_points_refuse_other_arguments():
     assert L.ssa_cache_append(ctypes.byref(c), None) == 0
 
 
+@pytest.mark.parametrize("T,R,Hq,Hkv,width,top", [
+    (1, 1, 32, 1, 1 << 14, 0), (1000, 1, 32, 1, 2048, 0), (70, 1, 8, 8, 1 << 14, 0),
+    (8192, 4, 32, 8, 512, 0), (1 << 17, 1, 32, 8, 2048, 0), (4096, 4096, 32, 8, 1 << 14, 0),
+    (300, 9, 64, 64, 4096, 0), (64, 64, 32, 8, 4096, 2048), (1 << 16, 8, 32, 1, 4096, 16)])
+def test_workspace_is_bounded(T, R, Hq, Hkv, width, top):
+    """Chunks are cut for about 2,048 workgroups: 128 columns of 258 floats each at
+    most, whatever the rows, the requests and the table's width."""
+    a = _lib.CachedAttentionArgs(
+        _c_cache(Hkv=Hkv, D=256, d=256), _c_rows(T=T, R=R, width=width, table_stride=width), 256,
+        256, _lib.SSA_BF16, Hq, Hq * 256, 256, Hq * 256, 256, 0.0625, 256 if top else None, top)
+    n = _lib.lib().ssa_cached_attention_workspace_bytes(ctypes.byref(a))
+    assert 0 <= n <= (2 * 2048 + 512) * 64 * 258 * 4
+
+
 # ---------------------------------------------------------------------------- page table
 def test_released_pages_return_once():
     t = ssa_amd.PageTable(4, 3, 10, 32, device="cpu")
@@ -246,7 +260,7 @@ def test_released_pages_return_once():
     held = [p for p in t.block_table.flatten().tolist() if p >= 0]
     assert sorted(t._free[:9].tolist() + held) == list(range(10))
     t.release(torch.tensor([], dtype=torch.int64))
-    t.release(torch.tensor([1]))
+    t.release(torch.tensor([1, 7, -1]))                   # 7 and -1 name no place
     assert sorted(t._free[:10].tolist()) == list(range(10)) and t.free_count.item() == 10
 
 

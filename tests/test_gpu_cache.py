@@ -418,6 +418,42 @@ def test_attention_with_scales_far_apart():
     _check_attend(c, b, q, qd)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("lens,new", [([20 * 32], [4]), ([20 * 32], [100]), ([640] * 2, [1, 1])])
+def test_attention_with_pages_of_zeros(dtype, lens, new):
+    """Pages whose values are all zero have the smallest scale there is; beside large
+    numbers, first, last and in between, they add nothing and lose nothing."""
+    ps, d = 32, 64
+    for size, zeros in ((40, (0, 7, 8, 19)), (-50, (3, 19)), (2, (0, 1, 2, 18, 19)), (6, (5,))):
+        c = _random_cache(40, 1, d, ps, 5)
+        b = _batch(lens, new, ps, 40, 5)
+        c.v_scale.fill_(2.0 ** size)
+        for r in range(len(lens)):
+            for p in zeros:
+                c.v_codes.view(torch.uint8)[b[0][r][p]] = 0
+                c.v_scale[b[0][r][p]] = 2.0 ** -100
+        q, qd = _queries(len(b[2]), 2, d, F32, 13)
+        if dtype == F16 and size > 10:
+            continue                                       # results beyond its range
+        _check_attend(c, b, q.to(dtype), qd.to(dtype))
+
+
+def test_attention_over_a_table_of_longer_rows():
+    """Block tables as a view of wider rows."""
+    ps, d = 32, 64
+    b = _batch([100, 300, 77], [1, 60, 3], ps, 30, 1)
+    c = _random_cache(30, 2, d, ps, 1)
+    q, qd = _queries(64, 4, d, BF16, 2)
+    want = _check_attend(c, b, q, qd)
+    wide = torch.full((3, 64), 10 ** 6, dtype=torch.int32, device=DEV)
+    w = len(b[0][0])
+    wide[:, 3:3 + w] = _i32(b[0])
+    plan = _plan(b)
+    plan.block_table = wide[:, 3:3 + w]
+    assert torch.equal(ssa_amd.cached_attention(qd, c, plan), want)
+    assert torch.equal(ssa_amd.select_pages(qd, c, plan, 2), ssa_amd.select_pages(qd, c, _plan(b), 2))
+
+
 def test_attention_writes_only_its_rows():
     """A given output of other strides; what lies around it stays."""
     ps, d = 64, 80
