@@ -688,14 +688,16 @@ int launch_select(const ssa_select_pages_args &a, hipStream_t s) {
 }
 
 // Few rows: a CU has one workgroup or none, and 16 waves shorten its walk over the
-// pages.  Many: a wave each, with no barriers to wait at (1,000 rows of 4 heads over 250
-// pages: 29 us with 4 waves), where the LDS holds enough of them.
+// pages (256 of up to 500 pages: 15 us, with 4 waves 18 us; 512: 26 us and 20 us).  Many:
+// a wave each, with no barriers to wait at (4,096 of 125 pages: 28 us, with 4 waves 33
+// us), where the LDS holds enough of them and no wave has so many pages that the chip
+// waits for the last ones (2,048 of 500: 81 us, with 4 waves 57 us; 4,096: 106 and 107).
 template <typename T, int D>
 int launch_select_d(const ssa_select_pages_args &a, hipStream_t s) {
     const int64_t n = (int64_t)a.rows.T * a.cache.Hkv;
-    if (n <= 512) return launch_select<T, D, 1024>(a, s);
-    return n > 2048 && a.rows.width <= 1024 ? launch_select<T, D, 64>(a, s)
-                                            : launch_select<T, D, 256>(a, s);
+    if (n <= 256) return launch_select<T, D, 1024>(a, s);
+    if (n >= 2048 && a.rows.width <= (n < 8192 ? n / 8 : 1024)) return launch_select<T, D, 64>(a, s);
+    return launch_select<T, D, 256>(a, s);
 }
 
 template <typename T>

@@ -5,7 +5,8 @@
 //     m' = max(m, max_j s_j),  a = 2^(m - m'),  p_j = 2^(s_j - m'),
 //     l' = a l + sum p_j,      O' = a O + p V     (s in units of log 2).
 //
-// Both products run on 16x16x32 bf16 MFMA, transposed: S^T = K Q^T and
+// Both products run on 16x16x32 MFMA (K Q^T in bf16, for fp16 queries in f16; V^T P^T
+// in f16, for fp32 queries in bf16), transposed: S^T = K Q^T and
 // O^T = V^T P^T, so that a column is one query row throughout and the C layout of
 // S^T is, lane for lane, the B layout of P^T.  That fixes which key a lane's rows
 // stand for: in a tile of KT keys, row 4g + r of block b is key KT/4 g + 4b + r,
@@ -15,15 +16,22 @@
 // Codes become 16-bit floats in one instruction for two, exactly (a code has 4
 // significant bits), and queries are exact too, so products are and only fp32 sums
 // round; probabilities round to 11 bits, for fp32 queries to 24.
+//
+// Single tokens are bound by reading codes: 16 over 16k to 32k keys (32 / 8 heads, d
+// 128, bf16) take 122 us, 4.7 TB/s, where a large copy reaches 4.8.  Chosen pages of a
+// prompt's rows are bound by the L2, each row having a list of its own.
 #include "ssa_cache_attend_dev.h"
 
 namespace {
 
-template <typename T, int D, int KT, int RT, bool SHARED>
-__global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE, D <= 128 && RT == 1 ? (SHARED || sizeof(T) == 4 ? 2 : 3) : 1)
+// A wave a unit fits three waves a SIMD (1,024 rows of 16 chosen pages: 134 us, with two
+// 147 us); four waves to a unit are better with two and more in flight each (16 tokens,
+// as above: 126 us, with three 151 us).
+template <typename T, int D, int KT, bool SHARED>
+__global__ void __launch_bounds__(ATT_WAVES * SSA_WAVE, D <= 128 ? (SHARED || sizeof(T) == 4 ? 2 : 3) : 1)
 cache_attend_kernel(AttendParams p) {
-    __shared__ u32x4 lds[attend_lds<D, KT, RT, SHARED>()];
-    attend_unit<T, D, KT, RT, SHARED>(p, blockIdx.x, (int)blockIdx.y, lds);
+    __shared__ u32x4 lds[attend_lds<D, KT, SHARED>()];
+    attend_unit<T, D, KT, SHARED>(p, blockIdx.x, (int)blockIdx.y, lds);
 }
 
 // Joins the chunks of each column: D / 4 lanes a column, four channels each.  Bound by
@@ -106,13 +114,15 @@ cache_join_kernel(AttendParams p, AttendParams q, int CT) {
 // What a call launches.  Many columns (rows times query heads of a kv head) of one
 // request share its keys, staged in LDS (ssa_cache_prompt.hip); single tokens are
 // bound by reading keys and go to the kernel above.  The lengths are on the GPU, so
-// the host goes by T / R alone: at most 4 rows a request on average, all go one way;
-// else all the other, where requests with at most MANY columns are cut into chunks of
-// their keys of their own, having few units each.
+// the host goes by T / R alone: at most 4 rows a request on average, all go one way
+// (32 requests of 2 rows over up to 8k keys 97 us, the other way 118 us; 4 requests of
+// 8 rows over up to 16k keys 59 us and 49 us; a prompt of 4,096 rows 514 us and 172
+// us); else all the other, where requests with at most MANY columns are cut into chunks
+// of their keys of their own, having few units each.
 constexpr int MANY = 64;
 
 struct AttendShape {
-    int RT, KT, mode, S, chunk;
+    int KT, mode, S, chunk;
     int64_t units;
     bool shared, prompt;
     int prompt_S, prompt_chunk, columns;      // columns: of a unit
@@ -136,9 +146,7 @@ AttendShape attend_shape(const ssa_cached_attention_args *a) {
     const int64_t T = a->rows.T, R = a->rows.R;
     const int rep = a->Hq / c.Hkv;
     s.KT = c.page < 64 ? 32 : 64;
-    // two tiles of heads share a wave's keys where the registers hold both
-    s.RT = rep > 16 && c.D <= 128 ? 2 : 1;
-    s.columns = 16 * s.RT;
+    s.columns = 16;
     s.shared = true;
     const int per_page = c.page / s.KT;
     int64_t tiles = (int64_t)a->rows.width * per_page;   // the most that a unit can have
@@ -162,7 +170,13 @@ AttendShape attend_shape(const ssa_cached_attention_args *a) {
     // 2,048 39.2 us).  Lengths are not: smaller chunks even them out (2,048: 16 tokens
     // over up to 32k keys 124 us, with 512 128 us, with 4,096 131 us).
     split_tiles(tiles, s.units * c.Hkv, a->pages ? 512 : 2048, 2 * ATT_WAVES, &s.S, &s.chunk);
-    if (!s.prompt && s.units * c.Hkv >= 4096) {
+    // A wave a unit, where there are units enough for that: over a few keys (256 tokens
+    // over 4 pages of 64: 31 us, with four waves to a unit 43 us; over 24 pages 150 us
+    // and 148 us), and where rows of one request, whose chosen pages are alike, run side
+    // by side in a workgroup and read them from its CU's cache (512 rows of 24 pages 108
+    // us, with four waves to a unit 139 us; 128 rows 48 us and 41 us).
+    const int64_t waves = s.units * c.Hkv;
+    if (!s.prompt && ((tiles * s.KT <= 512 && waves >= 1024) || (T > 4 * R && waves >= 2048))) {
         s.shared = false;
         s.S = 1;
         s.chunk = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
@@ -192,14 +206,14 @@ int check_attend(const ssa_cached_attention_args *a) {
     return SSA_OK;
 }
 
-template <typename T, int D, int KT, int RT>
+template <typename T, int D, int KT>
 void launch_attend(const AttendParams &p, const AttendShape &s, hipStream_t st) {
     if (s.shared) {
         const dim3 grid((unsigned)(p.units * p.Hkv), (unsigned)p.S);
-        cache_attend_kernel<T, D, KT, RT, true><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
+        cache_attend_kernel<T, D, KT, true><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
     } else {
         const unsigned grid = (unsigned)(ceil_div(p.units, ATT_WAVES) * p.Hkv);
-        cache_attend_kernel<T, D, KT, RT, false><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
+        cache_attend_kernel<T, D, KT, false><<<grid, ATT_WAVES * SSA_WAVE, 0, st>>>(p);
     }
 }
 
@@ -228,14 +242,8 @@ void launch_attend_d(const AttendParams &p, const AttendShape &s, hipStream_t st
         ssa_cache_prompt_launch(p, q, dtype, D, s.KT, st);
         return launch_join<T, D>(p, q, s, st);
     }
-    if constexpr (D <= 128)
-        if (s.RT == 2) {
-            if (s.KT == 32) launch_attend<T, D, 32, 2>(p, s, st);
-            else launch_attend<T, D, 64, 2>(p, s, st);
-            return launch_join<T, D>(p, q, s, st);
-        }
-    if (s.KT == 32) launch_attend<T, D, 32, 1>(p, s, st);
-    else launch_attend<T, D, 64, 1>(p, s, st);
+    if (s.KT == 32) launch_attend<T, D, 32>(p, s, st);
+    else launch_attend<T, D, 64>(p, s, st);
     launch_join<T, D>(p, q, s, st);
 }
 

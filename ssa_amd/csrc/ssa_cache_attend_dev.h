@@ -180,7 +180,7 @@ template <> struct Ops<float> {
 //    smallest scale there is) are taken as zeros: O in their units could leave fp32.
 // For fp32 queries p is three bf16 terms (24 bits; V scaled, as bf16 holds every
 // scale).
-template <typename T, int D, int KT, int RT>
+template <typename T, int D, int KT>
 struct Columns {
     typedef Ops<T> O_;
     typedef typename O_::Q QV;
@@ -192,14 +192,14 @@ struct Columns {
     static constexpr int ROOM = F32 ? 0 : 5, LIFT = 6;
     static constexpr float GROWN = 4.f;
 
-    QV q[RT][DP * 2][NQ];
-    f32x4 o[RT][ND], l[RT];
-    float m[RT], scale;
+    QV q[DP * 2][NQ];
+    f32x4 o[ND], l;
+    float m, scale;
     int e_ref, e_top;            // O's unit; the largest it has been
-    int pos[RT];                 // last key a column sees; none for it to lose if it is dead
+    int pos;                     // last key a column sees; none for it to lose if it is dead
     int most, least;             // of the live columns
 
-    // columns c0 + 16 rt + lane % 16 below c1 of unit u, kv head h
+    // columns c0 + lane % 16 below c1 of unit u, kv head h
     __device__ __forceinline__ void start(const AttendParams &p, const Unit &u, int c0, int c1, int h) {
         const int lane = lane_id(), col = lane & 15, g = lane >> 4;
         const bool neg = p.scale < 0.f;
@@ -207,52 +207,49 @@ struct Columns {
         e_ref = e_top = -10000;  // anything is larger, and O is 0
         most = -1;
         least = 0x7fffffff;
+        const int c = c0 + col;
+        const bool live = c < c1;
+        // dead lanes load the last live column, so that no load waits for another
+        const int cc = min(c, c1 - 1), t = u.t0 + cc / p.rep;
+        const int32_t req = p.requests[t], at = p.positions[t];
+        const int seen = live && u.req >= 0 && req == u.req ? at : -1;
+        most = max(most, seen);
+        if (live) least = min(least, seen);
+        pos = live ? seen : 0x7fffffff;
+        const T *row = (const T *)p.q + t * p.q_st + (int64_t)(h * p.rep + cc % p.rep) * p.q_sh;
+        T raw[DP * 2][8];
+        if (p.q_vec) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int c = c0 + rt * 16 + col;
-            const bool live = c < c1;
-            // dead lanes load the last live column, so that no load waits for another
-            const int cc = min(c, c1 - 1), t = u.t0 + cc / p.rep;
-            const int32_t req = p.requests[t], at = p.positions[t];
-            const int seen = live && u.req >= 0 && req == u.req ? at : -1;
-            most = max(most, seen);
-            if (live) least = min(least, seen);
-            pos[rt] = live ? seen : 0x7fffffff;
-            const T *row = (const T *)p.q + t * p.q_st + (int64_t)(h * p.rep + cc % p.rep) * p.q_sh;
-            T raw[DP * 2][8];
-            if (p.q_vec) {
-#pragma unroll
-                for (int s = 0; s < DP * 2; ++s) {
-                    const int x = (s >> 1) * 64 + g * 16 + (s & 1) * 8;
-                    __builtin_memcpy(raw[s], __builtin_assume_aligned(row + (x < p.d ? x : 0), 16),
-                                     sizeof(raw[s]));
-                }
-            } else {
-#pragma unroll
-                for (int s = 0; s < DP * 2; ++s)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        raw[s][j] = row[min((s >> 1) * 64 + g * 16 + (s & 1) * 8 + j, p.d - 1)];
+            for (int s = 0; s < DP * 2; ++s) {
+                const int x = (s >> 1) * 64 + g * 16 + (s & 1) * 8;
+                __builtin_memcpy(raw[s], __builtin_assume_aligned(row + (x < p.d ? x : 0), 16),
+                                 sizeof(raw[s]));
             }
+        } else {
 #pragma unroll
             for (int s = 0; s < DP * 2; ++s)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int x = (s >> 1) * 64 + g * 16 + (s & 1) * 8 + j;
-                    float v = to_f32(raw[s][j]);
-                    v = live && x < p.d ? (neg ? -v : v) : 0.f;
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) {
-                        const typename O_::QE b = (typename O_::QE)v;
-                        q[rt][s][n][j] = b;
-                        v -= (float)b;
-                    }
-                }
-            m[rt] = -INFINITY;
-            l[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < ND; ++i) o[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < 8; ++j)
+                    raw[s][j] = row[min((s >> 1) * 64 + g * 16 + (s & 1) * 8 + j, p.d - 1)];
         }
+#pragma unroll
+        for (int s = 0; s < DP * 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int x = (s >> 1) * 64 + g * 16 + (s & 1) * 8 + j;
+                float v = to_f32(raw[s][j]);
+                v = live && x < p.d ? (neg ? -v : v) : 0.f;
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    const typename O_::QE b = (typename O_::QE)v;
+                    q[s][n][j] = b;
+                    v -= (float)b;
+                }
+            }
+        m = -INFINITY;
+        l = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         most = (int)wave_max_u((uint32_t)(most + 1)) - 1;
         most = min(most, (p.width << p.page_shift) - 1);
         least = (int)wave_min_u((uint32_t)(least + 1)) - 1;
@@ -260,82 +257,64 @@ struct Columns {
 
     // scores to probabilities: key scale ks, value scale vs, first key of the tile;
     // l takes their sums.  False where the tile's values count as zeros.
-    __device__ __forceinline__ bool softmax(f32x4 (&s)[RT][NB], float ks, float vs, int key0,
-                                             PV (&pf)[RT][KS][NP]) {
+    __device__ __forceinline__ bool softmax(f32x4 (&s)[NB], float ks, float vs, int key0,
+                                            PV (&pf)[KS][NP]) {
         const int g = lane_id() >> 4;
         float c = scale * ks;                 // log2 units of a score's unit
         if (key0 + KT - 1 > least) {          // some column ends in this tile
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        s[rt][b][r] = key0 + KT / 4 * g + 4 * b + r <= pos[rt] ? s[rt][b][r] * c
-                                                                              : -INFINITY;
+                for (int r = 0; r < 4; ++r)
+                    s[b][r] = key0 + KT / 4 * g + 4 * b + r <= pos ? s[b][r] * c : -INFINITY;
             c = 1.f;
         }
         const int ev = F32 ? 0 : (int)(__builtin_amdgcn_readfirstlane(__float_as_uint(vs)) >> 23) - 127;
-        float mx[RT];
-        bool grow = false;
+        float mx = s[0][0];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float v = s[rt][0][0];
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v = fmaxf(v, s[rt][b][r]);
-            mx[rt] = v * c;
-            grow |= mx[rt] > m[rt] + GROWN;
-        }
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[b][r]);
+        mx *= c;
         const bool tiny = !F32 && ev < e_top - 64;
         const bool move = !tiny && (ev > e_ref + LIFT || ev < e_ref);
-        if (wave_ballot(grow) || move) {
+        if (wave_ballot(mx > m + GROWN) || move) {
             const int e_new = move ? (F32 ? 0 : ev - 3) : e_ref;
             const float unit = __builtin_amdgcn_exp2f((float)(e_ref - e_new));
             e_ref = e_new;
             e_top = max(e_top, e_new);
+            float v = fmaxf(mx, __shfl_xor(mx, 16, SSA_WAVE));
+            v = fmaxf(v, __shfl_xor(v, 32, SSA_WAVE));
+            v = fmaxf(v, m);
+            const float a = __builtin_amdgcn_exp2f(m - (v == -INFINITY ? 0.f : v));
+            m = v;
+            l *= a;
+            const float au = a * unit;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                float v = mx[rt];
-                v = fmaxf(v, __shfl_xor(v, 16, SSA_WAVE));
-                v = fmaxf(v, __shfl_xor(v, 32, SSA_WAVE));
-                v = fmaxf(v, m[rt]);
-                const float a = __builtin_amdgcn_exp2f(m[rt] - (v == -INFINITY ? 0.f : v));
-                m[rt] = v;
-                l[rt] *= a;
-                const float au = a * unit;
-#pragma unroll
-                for (int i = 0; i < ND; ++i) o[rt][i] *= au;
-            }
+            for (int i = 0; i < ND; ++i) o[i] *= au;
         }
         const float lift = (float)(tiny ? ROOM : ev - e_ref + ROOM);
+        const float sub = lift - (m == -INFINITY ? 0.f : m);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const float sub = lift - (m[rt] == -INFINITY ? 0.f : m[rt]);
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int r = 0; r < 4; ++r) {
+                float v = __builtin_amdgcn_exp2f(fmaf(s[b][r], c, sub));
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float v = __builtin_amdgcn_exp2f(fmaf(s[rt][b][r], c, sub));
-#pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        const typename O_::PE e = (typename O_::PE)v;
-                        pf[rt][b >> 1][n][(b & 1) * 4 + r] = e;
-                        if (n + 1 < NP) v -= (float)e;
-                    }
+                for (int n = 0; n < NP; ++n) {
+                    const typename O_::PE e = (typename O_::PE)v;
+                    pf[b >> 1][n][(b & 1) * 4 + r] = e;
+                    if (n + 1 < NP) v -= (float)e;
                 }
-        }
+            }
         PV ones;
         const typename O_::PE one = (typename O_::PE)__builtin_amdgcn_exp2f(-lift);
 #pragma unroll
         for (int j = 0; j < 8; ++j) ones[j] = one;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int n = NP - 1; n >= 0; --n) l[rt] = mfma(ones, pf[rt][k][n], l[rt]);
+            for (int n = NP - 1; n >= 0; --n) l = mfma(ones, pf[k][n], l);
         return !tiny;
     }
 
@@ -346,72 +325,70 @@ struct Columns {
                                            int split, bool any) {
         const int lane = lane_id(), col = lane & 15, g = lane >> 4;
         const float un = unit();
+        const int c = c0 + col;
+        if (c >= c1) return;
+        const int t = u.t0 + c / p.rep, hq = h * p.rep + c % p.rep;
+        const float sum = l[0];
+        if (p.S == 1) {
+            T *row = (T *)p.out + t * p.o_st + hq * p.o_sh;
+            const float f = sum == 0.f ? 0.f : un / sum;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int c = c0 + rt * 16 + col;
-            if (c >= c1) continue;
-            const int t = u.t0 + c / p.rep, hq = h * p.rep + c % p.rep;
-            const float sum = l[rt][0];
-            if (p.S == 1) {
-                T *row = (T *)p.out + t * p.o_st + hq * p.o_sh;
-                const float f = sum == 0.f ? 0.f : un / sum;
+            for (int i = 0; i < ND; ++i) {
+                const int x = i * 16 + 4 * g;
+                T v[4];
 #pragma unroll
-                for (int i = 0; i < ND; ++i) {
-                    const int x = i * 16 + 4 * g;
-                    T v[4];
+                for (int r = 0; r < 4; ++r)
+                    Cvt<T>::store(v + r, sum == 0.f ? 0.f : o[i][r] * f);
+                if (p.o_vec) {
+                    if (x < p.d)
+                        __builtin_memcpy(__builtin_assume_aligned(row + x, 4 * sizeof(T)), v, sizeof(v));
+                } else {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        Cvt<T>::store(v + r, sum == 0.f ? 0.f : o[rt][i][r] * f);
-                    if (p.o_vec) {
-                        if (x < p.d)
-                            __builtin_memcpy(__builtin_assume_aligned(row + x, 4 * sizeof(T)), v,
-                                             sizeof(v));
-                    } else {
+                        if (x + r < p.d) row[x + r] = v[r];
+                }
+            }
+        } else {
+            const int64_t at = part_of(p, u, c, h) + split;
+            if (any) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (x + r < p.d) row[x + r] = v[r];
-                    }
-                }
-            } else {
-                const int64_t at = part_of(p, u, c, h) + split;
-                if (any) {
-#pragma unroll
-                    for (int i = 0; i < ND; ++i)
-                        *(f32x4 *)(p.part_o + at * D + i * 16 + 4 * g) = o[rt][i] * un;
-                }
-                if (g == 0) {
-                    p.part_ml[2 * at] = m[rt];
-                    p.part_ml[2 * at + 1] = sum;
-                }
+                for (int i = 0; i < ND; ++i)
+                    *(f32x4 *)(p.part_o + at * D + i * 16 + 4 * g) = o[i] * un;
+            }
+            if (g == 0) {
+                p.part_ml[2 * at] = m;
+                p.part_ml[2 * at + 1] = sum;
             }
         }
     }
 };
 
-// A unit is 16 RT columns.  SHARED: a workgroup takes one unit and a chunk of its key
-// tiles, its waves every fourth tile, and their sums are joined in LDS.  Otherwise
-// each wave takes a unit of its own and all of its tiles: no joining, for calls with
-// units enough to fill the chip.  A wave holds one tile's values and the next one's
-// keys in flight, and looks page ids up a tile ahead of those.
-// 16-byte pieces of LDS it uses
-template <int D, int KT, int RT, bool SHARED>
+// 16-byte pieces of LDS that attend_unit uses
+template <int D, int KT, bool SHARED>
 constexpr int attend_lds() {
-    const int moving = ATT_WAVES * KT * D / 16, joined = SHARED ? 16 * RT * (D + 4) / 4 : 0;
-    return (moving > joined ? moving : joined) + ATT_WAVES * 16 * RT / 2;
+    const int moving = ATT_WAVES * KT * D / 16, joined = SHARED ? 16 * (D + 4) / 4 : 0;
+    return (moving > joined ? moving : joined) + ATT_WAVES * 16 / 2;
 }
 
-template <typename T, int D, int KT, int RT, bool SHARED>
+// A unit is 16 columns.  SHARED: a workgroup takes one unit and a chunk of its key
+// tiles, its waves every fourth tile, and their sums are joined in LDS.  Otherwise
+// each wave takes a unit of its own and all of its tiles, and nothing is joined.  A
+// wave holds one tile's values and the next one's keys in flight, and looks page ids
+// up a tile ahead of those.  (Units of 32 columns, for more than 16 query heads of a
+// kv head, read their keys once and not twice, but a wave then holds twice the state
+// and waits more: 64 tokens of 32 heads over one, 4k to 8k keys, 101 us to 65 us.)
+template <typename T, int D, int KT, bool SHARED>
 __device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned block, int split,
                                             u32x4 *lds) {
-    typedef Columns<T, D, KT, RT> C;
+    typedef Columns<T, D, KT> C;
     typedef typename C::PV PV;
     constexpr int NQ = C::NQ, NP = C::NP, NB = C::NB, DP = C::DP, ND = C::ND, KS = C::KS;
-    constexpr int CT = 16 * RT, OS = D + 4;   // OS: row stride of the joined sums
+    constexpr int CT = 16, OS = D + 4;        // OS: row stride of the joined sums
     // each wave's pieces on their way to other lanes; then the joined sums
     u32x4 *x_lds = lds;
     constexpr int XW = KT * D / 16;
     float *o_lds = (float *)lds;
-    float (*m_lds)[CT] = (float (*)[CT])(lds + attend_lds<D, KT, RT, SHARED>() - ATT_WAVES * CT / 2);
+    float (*m_lds)[CT] = (float (*)[CT])(lds + attend_lds<D, KT, SHARED>() - ATT_WAVES * CT / 2);
     float (*l_lds)[CT] = m_lds + ATT_WAVES;
 
     const int lane = lane_id(), col = lane & 15, g = lane >> 4;
@@ -502,28 +479,25 @@ __device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned bloc
 #pragma unroll
                 for (int i = 0; i < DP; ++i) kr[b][i] = xk[(b * DP + i) * SSA_WAVE + from];
             __builtin_amdgcn_sched_barrier(0);
-            f32x4 s[RT][NB];
+            f32x4 s[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) s[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+                s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < DP; ++i) {
                     const u32x4 x = kr[b][i];
                     const typename C::QV k0 = Ops<T>::key(x.x, x.y), k1 = Ops<T>::key(x.z, x.w);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int n = NQ - 1; n >= 0; --n) {
-                            s[rt][b] = mfma(k0, w.q[rt][2 * i][n], s[rt][b]);
-                            s[rt][b] = mfma(k1, w.q[rt][2 * i + 1][n], s[rt][b]);
-                        }
+                    for (int n = NQ - 1; n >= 0; --n) {
+                        s[b] = mfma(k0, w.q[2 * i][n], s[b]);
+                        s[b] = mfma(k1, w.q[2 * i + 1][n], s[b]);
+                    }
                 }
             }
             pg1 = place(tile + STEP, lp1, entry1);
             fetch_keys(tile + STEP, pg1);
             __builtin_amdgcn_sched_barrier(0);
-            PV pf[RT][KS][NP];
+            PV pf[KS][NP];
             const bool some = w.softmax(s, kscale, vscale, (lp << p.page_shift) + sub * KT, pf);
             wave_lds_sync();
             if (some) {
@@ -552,10 +526,8 @@ __device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned bloc
                     for (int k = 0; k < KS; ++k) {
                         const PV vf = Ops<T>::value(vr[i][2 * k], vr[i][2 * k + 1], vscale);
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                            for (int n = NP - 1; n >= 0; --n)
-                                w.o[rt][i] = mfma(vf, pf[rt][k][n], w.o[rt][i]);
+                        for (int n = NP - 1; n >= 0; --n)
+                            w.o[i] = mfma(vf, pf[k][n], w.o[i]);
                     }
             }
             wave_lds_sync();
@@ -574,27 +546,22 @@ __device__ __forceinline__ void attend_unit(const AttendParams &p, unsigned bloc
     }
 
     // join the waves: m, l, O in the waves' order
-    if (g == 0)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            m_lds[wave][rt * 16 + col] = w.m[rt];
-            l_lds[wave][rt * 16 + col] = w.l[rt][0];
-        }
+    if (g == 0) {
+        m_lds[wave][col] = w.m;
+        l_lds[wave][col] = w.l[0];
+    }
     __syncthreads();                          // (and no wave's pieces are read any more)
     const float unit = w.unit();
     for (int v = 0; v < ATT_WAVES; ++v) {
         if (v == wave) {
+            float mx = -INFINITY;
+            for (int i = 0; i < ATT_WAVES; ++i) mx = fmaxf(mx, m_lds[i][col]);
+            const float a = __builtin_amdgcn_exp2f(w.m - (mx == -INFINITY ? 0.f : mx)) * unit;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                float mx = -INFINITY;
-                for (int i = 0; i < ATT_WAVES; ++i) mx = fmaxf(mx, m_lds[i][rt * 16 + col]);
-                const float a = __builtin_amdgcn_exp2f(w.m[rt] - (mx == -INFINITY ? 0.f : mx)) * unit;
-#pragma unroll
-                for (int i = 0; i < ND; ++i) {
-                    f32x4 *at = (f32x4 *)&o_lds[(rt * 16 + col) * OS + i * 16 + 4 * g];
-                    const f32x4 x = w.o[rt][i] * a;
-                    *at = v == 0 ? x : *at + x;
-                }
+            for (int i = 0; i < ND; ++i) {
+                f32x4 *at = (f32x4 *)&o_lds[col * OS + i * 16 + 4 * g];
+                const f32x4 x = w.o[i] * a;
+                *at = v == 0 ? x : *at + x;
             }
         }
         __syncthreads();

@@ -3,7 +3,7 @@
 //
 // The products and the mapping of keys to lanes are those of ssa_cache_attend.hip
 // (S^T = K Q^T, O^T = V^T P^T, a column is a query row, P^T stays in registers).
-// Here each wave owns 16 RT columns and walks every key tile of the workgroup's
+// Here each wave owns 16 columns and walks every key tile of the workgroup's
 // range, so the tiles are shared: the waves convert a tile's codes to 16-bit floats
 // once, into LDS, in the order in which the matrix operands read them (a fragment is
 // 64 slots of 16 bytes: every LDS access is free of conflicts), double-buffered, with
@@ -26,12 +26,12 @@ template <typename T, int D> constexpr int prompt_waves() { return sizeof(T) == 
 
 template <typename T, int D, int KT>
 __device__ __forceinline__ void prompt_unit(const AttendParams &p, unsigned block, int split, u32x4 *lds) {
-    constexpr int RT = 1, PW = prompt_waves<T, D>();
-    typedef Columns<T, D, KT, RT> C;
+    constexpr int PW = prompt_waves<T, D>();
+    typedef Columns<T, D, KT> C;
     typedef typename C::QV QV;
     typedef typename C::PV PV;
     constexpr int NQ = C::NQ, NP = C::NP, NB = C::NB, DP = C::DP, ND = C::ND, KS = C::KS;
-    constexpr int CT = PW * 16 * RT;
+    constexpr int CT = PW * 16;
     // a load unit: 16 codes a lane, two fragments
     constexpr int KU = NB * DP, VU = ND * KS / 2, NU = KU + VU, UW = NU < PW ? 1 : NU / PW;
     u32x4 (*frag)[2 * NU][SSA_WAVE] = (u32x4 (*)[2 * NU][SSA_WAVE])lds;    // two buffers
@@ -46,7 +46,7 @@ __device__ __forceinline__ void prompt_unit(const AttendParams &p, unsigned bloc
     const int u = p.units - 1 - (int)(block / (unsigned)p.Hkv);
     Unit un;
     if (!locate_unit(p, u, CT, un)) return;
-    const int wc0 = un.c0 + wave * 16 * RT;   // this wave's first column
+    const int wc0 = un.c0 + wave * 16;        // this wave's first column
     C w;
     w.start(p, un, wc0, un.c1, h);
     if (lane == 0) most_lds[wave] = w.most;
@@ -141,11 +141,9 @@ __device__ __forceinline__ void prompt_unit(const AttendParams &p, unsigned bloc
         entry3 = entry(tile + 4);
         const int key0 = tile * KT;
         if (cur.pg >= 0 && key0 <= w.most) {
-            f32x4 s[RT][NB];
+            f32x4 s[NB];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int b = 0; b < NB; ++b) s[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int b = 0; b < NB; ++b) s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
             const u32x4 *kl = &frag[buf][0][from], *vl = &frag[buf][2 * KU][from];
 #pragma unroll
             for (int k = 0; k < DP * 2; ++k)   // neighbouring products are independent
@@ -153,9 +151,9 @@ __device__ __forceinline__ void prompt_unit(const AttendParams &p, unsigned bloc
                 for (int b = 0; b < NB; ++b) {
                     const QV kf = *(const QV *)(kl + (b * DP * 2 + k) * SSA_WAVE);
 #pragma unroll
-                    for (int n = NQ - 1; n >= 0; --n) s[0][b] = mfma(kf, w.q[0][k][n], s[0][b]);
+                    for (int n = NQ - 1; n >= 0; --n) s[b] = mfma(kf, w.q[k][n], s[b]);
                 }
-            PV pf[1][KS][NP];
+            PV pf[KS][NP];
             if (w.softmax(s, cur.ks, cur.vs, key0, pf))
 #pragma unroll
                 for (int i = 0; i < ND; ++i)
@@ -163,7 +161,7 @@ __device__ __forceinline__ void prompt_unit(const AttendParams &p, unsigned bloc
                     for (int k = 0; k < KS; ++k) {
                         const PV vf = *(const PV *)(vl + (i * KS + k) * SSA_WAVE);
 #pragma unroll
-                        for (int n = NP - 1; n >= 0; --n) w.o[0][i] = mfma(vf, pf[0][k][n], w.o[0][i]);
+                        for (int n = NP - 1; n >= 0; --n) w.o[i] = mfma(vf, pf[k][n], w.o[i]);
                     }
         }
         __syncthreads();
