@@ -539,6 +539,18 @@ def test_attention_over_chosen_pages_for_many_rows(dtype, Hq, H, d, ps):
     _check_attend(c, b, q, qd, pages=pages)
 
 
+@pytest.mark.parametrize("Hq,H,d,ps,top", [(4, 2, 64, 64, 20), (33, 1, 128, 64, 9)])
+def test_attention_over_many_chosen_pages_of_a_prompt(Hq, H, d, ps, top):
+    """More keys a row than a wave takes alone, but rows of one request side by side."""
+    T = 2050 // H
+    b = _batch([25 * ps + T, 7], [T, 1], ps, 27 + T // ps, d)
+    c = _random_cache(27 + T // ps, H, d, ps, d)
+    g = _gen(Hq)
+    pages = torch.stack([torch.randperm(24, generator=g)[:top] for _ in range((T + 1) * H)])
+    q, qd = _queries(T + 1, Hq, d, BF16, 4)
+    _check_attend(c, b, q, qd, pages=pages.reshape(T + 1, H, top).int())
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("Hq,H,d,ps", [(4, 4, 64, 32), (8, 2, 128, 64), (6, 1, 256, 128)])
 def test_attention_of_a_prompt_behind_a_long_context(dtype, Hq, H, d, ps):
@@ -593,6 +605,18 @@ def test_select_of_many_rows():
     q, qd = _queries(len(b[2]), 8, d, BF16, 2)
     got = ssa_amd.select_pages(qd, c, _plan(b), 7, first=2, recent=2)
     assert torch.equal(got.cpu(), ref.select(q, ref.Cache.of(c), b[0], b[2], b[3], 7, 2, 2))
+
+
+@pytest.mark.parametrize("rows", [255, 256, 257, 511, 512])
+def test_select_at_the_bounds_of_its_forms(rows):
+    """Rows times kv heads (1 and 4) and table widths on both sides of each rule."""
+    ps, d = 32, 64
+    for H, Hq, width in ((1, 2, None), (4, 4, None), (4, 4, 600)):
+        b = _batch([40 * ps + 3, 700], [rows - 30, 30], ps, 70, rows, width=width)
+        c = _random_cache(70, H, d, ps, rows)
+        q, qd = _queries(rows, Hq, d, BF16, H)
+        got = ssa_amd.select_pages(qd, c, _plan(b), 7, first=1, recent=2)
+        assert torch.equal(got.cpu(), ref.select(q, ref.Cache.of(c), b[0], b[2], b[3], 7, 1, 2))
 
 
 @pytest.mark.parametrize("R", [256, 257, 1024, 1025, 4096, 4097])
