@@ -534,9 +534,10 @@ class SparseAttention(nn.Module):
         budget = self.page_budget(cache.page_size) if sparse else None
         T = x.shape[0]
         q = self.Wq(x).view(T, self.H, self.d_head)
-        kv = F.linear(x, self._fused_weight((self.Wk, self.Wv))).view(T, 2 * self.n_kv,
-                                                                     self.d_head)
-        cache_append(cache, kv[:, :self.n_kv], kv[:, self.n_kv:], plan.slots)
+        # not the stacked weight of forward: a captured step must read the weights
+        # themselves, which a replay may find changed, and no copy that can go away
+        k, v = (w(x).view(T, self.n_kv, self.d_head) for w in (self.Wk, self.Wv))
+        cache_append(cache, k, v, plan.slots)
         pages = None
         if budget is not None:
             pages = select_pages(q, cache, plan, budget[0], first=budget[1], recent=budget[2])

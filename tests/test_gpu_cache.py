@@ -280,6 +280,23 @@ def test_select_over_many_pages(n_pages):
         assert torch.equal(got.cpu(), want), top
 
 
+@pytest.mark.parametrize("rows", [1, 300])
+def test_select_over_the_widest_table(rows):
+    """16,384 pages a request (the same ones again and again), in both forms that
+    take them."""
+    ps, d, H, W = 32, 64, 1, 16384
+    table = torch.randint(0, 900, (1, W), generator=_gen(rows))
+    req, pos = [0] * rows, [W * ps - rows + i for i in range(rows)]
+    c = _random_cache(900, H, d, ps, 3)
+    q, qd = _queries(rows, 2, d, F16, 6)
+    plan = _plan((table.tolist(), [0, rows], req, pos))
+    got = ssa_amd.select_pages(qd, c, plan, 33, first=1, recent=2)
+    few = [0, rows - 1]
+    want = ref.select(q[few], ref.Cache.of(c), table.tolist(), [0, 0], [pos[i] for i in few],
+                      33, 1, 2)
+    assert torch.equal(got[few].cpu(), want[:len(few)])
+
+
 def test_select_ties_missing_pages_and_nan():
     """Equal pages go to the lowest, absent pages come last, a page with a bad
     token first; a query that is NaN or zero takes the lowest pages."""
@@ -742,6 +759,47 @@ def test_captured_step_replays():
             assert torch.equal(x, y), (i, n)
         assert torch.equal(captured[1].lengths, eager[1].lengths)
     _same_cache(captured[0], ref.Cache.of(eager[0]))
+
+
+@torch.no_grad()
+def test_captured_layer_step_reads_the_weights_themselves():
+    """The first call of a layer under capture, its weights changed in place later and
+    eager calls between the replays: each replay is the eager step of a layer with the
+    weights of that moment."""
+    T, R, ps = 6, 3, 32
+
+    def make():
+        attn = _layer()
+        return attn, attn.new_cache(40, ps), ssa_amd.PageTable(R, 12, 40, ps, device=DEV)
+
+    def step(attn, cache, table, x, new):
+        return attn.forward_cached(x, cache, table.plan(new, T))
+
+    x, new = torch.zeros(T, 256, device=DEV), _i32([2] * R)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*make(), x, new)                              # another layer of the same sizes
+    torch.cuda.current_stream().wait_stream(side)
+    captured, eager = make(), make()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = step(*captured, x, new)
+    for i in range(12):
+        if i % 3 == 2:
+            for attn in (captured[0], eager[0]):
+                for n, w in enumerate((attn.Wq, attn.Wk, attn.Wv, attn.Wo)):
+                    w.weight.copy_(torch.randn(w.weight.shape, generator=_gen(9 * i + n)) / 16)
+        x.copy_(torch.randn(T, 256, generator=_gen(i)))
+        new.copy_(_i32([1, 2, i % 4]))
+        want = step(*eager, x, new)
+        torch.cuda.synchronize()
+        gr.replay()
+        junk = [torch.full((512, 256), float("nan"), device=DEV) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        del junk
+    _same_cache(captured[1], ref.Cache.of(eager[1]))
 
 
 def test_calls_on_another_stream():
