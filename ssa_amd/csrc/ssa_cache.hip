@@ -154,9 +154,9 @@ int launch_plan(const ssa_page_plan_args &a, hipStream_t s) {
 // rounded), then the codes, staged in LDS so that the transposed value codes go
 // out 16 tokens at a time.  D / 8 lanes hold a row, 8 columns each, and keep it in
 // registers between the two.  Bound by latency for single tokens (about five
-// dependent steps: 64 tokens of 8 heads 6.6 us).  A prompt (2,731 tokens of 8 heads, d
-// 96 in fp16) takes 24 us, 1.6 TB/s: a CU has one or two of these workgroups, whose
-// first pass waits for HBM before the second can start.
+// dependent steps: 64 tokens of 8 heads 6.6 us).  Prompts (8,193 rows of 8 heads, d
+// 96 in fp16) take 23 us, 1.7 TB/s: bound by the wait for the rows, all of a
+// workgroup's at once and two workgroups a CU (without forming codes 21 us).
 
 // Eight adjacent columns of a row, in the registers they take as they are stored.
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
@@ -171,7 +171,10 @@ template <typename T> struct Row8 {                        // 16-bit types
         w[j >> 1] = j & 1 ? (w[j >> 1] & 0xffffu) | (uint32_t)t.x << 16 : (uint32_t)t.x;
     }
     __device__ __forceinline__ void load(const T *p) { w = *(const u32x4 *)p; }
-    __device__ __forceinline__ void clear() { w = u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void cut(int n) {           // keeps the first n columns
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = n >= 2 * j + 2 ? w[j] : (n > 2 * j ? w[j] & 0xffffu : 0u);
+    }
 };
 template <> struct Row8<float> {
     u32x4 w[2];
@@ -181,20 +184,22 @@ template <> struct Row8<float> {
         w[0] = *(const u32x4 *)p;
         w[1] = *(const u32x4 *)(p + 4);
     }
-    __device__ __forceinline__ void clear() { w[0] = w[1] = u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void cut(int n) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j >> 2][j & 3] = n > j ? w[j >> 2][j & 3] : 0u;
+    }
 };
 
-// columns x .. x + 7 of a row, zeros past d.  VEC: d and the strides are multiples
+// columns x .. x + 7 of a row, anything past d.  VEC: d and the strides are multiples
 // of 8 (the addresses of 16 bytes)
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_row8(const void *p, int64_t at, int x, int d, Row8<T> &v) {
     const T *q = (const T *)p + at;
     if (VEC) {
         v.load(q + (x < d ? x : 0));
-        if (x >= d) v.clear();
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v.set(j, x + j < d ? q[x + j] : T{});
+        for (int j = 0; j < 8; ++j) v.set(j, q[min(x + j, d - 1)]);
     }
 }
 
@@ -205,6 +210,18 @@ __device__ __forceinline__ uint32_t max_bits8(const Row8<T> &v) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v.get(j)) & 0x7fffffffu);
     return m;
+}
+// the largest of N adjacent lanes' values (8, 16 or 32), in the vector unit: no lane
+// permutation by way of the LDS, whose latency a row's steps would add up to
+template <int N>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    auto with = [&](int u) { v = max(v, (uint32_t)u); };
+    with(__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true));      // lane ^ 1
+    with(__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true));      // lane ^ 2
+    with(__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));     // 7 - lane: the other four
+    if (N >= 16) with(__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true));   // 15 - lane
+    if (N >= 32) with(__shfl_xor((int)v, 16, SSA_WAVE));
+    return v;
 }
 template <typename T>
 __device__ __forceinline__ uint2 codes8(const Row8<T> &v, float f) {
@@ -285,12 +302,9 @@ cache_append_kernel(ssa_cache_append_args a, int window) {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
             if (i > 0 && i * RPW >= n) break;
-            uint32_t km = max_bits8(kv[i]), vm = max_bits8(vv[i]);
-#pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) {
-                km = max(km, (uint32_t)__shfl_xor((int)km, o, SSA_WAVE));
-                vm = max(vm, (uint32_t)__shfl_xor((int)vm, o, SSA_WAVE));
-            }
+            kv[i].cut(d - rx);         // here, so that no load above waits for another
+            vv[i].cut(d - rx);
+            const uint32_t km = lanes_max<LPR>(max_bits8(kv[i])), vm = lanes_max<LPR>(max_bits8(vv[i]));
             const int r = r0 + i * RPW;
             if (rx == 0 && r < n) {
                 kmax[r] = km;
@@ -476,7 +490,7 @@ int launch_append_t(const ssa_cache_append_args &a, hipStream_t s) {
 // each step.  The smallest taken key is then found by its digits, from the highest
 // bit in which keys differ, and the chosen pages are written in ascending order.
 // Bound by latency (page ids, then bounds: 32 rows of 8 heads over up to 512 pages 14
-// us) and by the conversions to fp64 (1,000 rows of 4 heads over 235 pages: 29 us).
+// us) and by the conversions to fp64 (1,000 rows of 4 heads over 250 pages: 27 us).
 constexpr int SEL_MAX_WIDTH = 16384;        // scores of a row in LDS
 
 // order-preserving map of a score: NaN as +inf, an absent page 0

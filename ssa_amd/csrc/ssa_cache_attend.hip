@@ -17,7 +17,7 @@
 // significant bits), and queries are exact too, so products are and only fp32 sums
 // round; probabilities round to 11 bits, for fp32 queries to 24.
 //
-// Single tokens are bound by reading codes: 16 over 16k to 32k keys (32 / 8 heads, d
+// Single tokens are bound by reading codes: 16 over 5k to 32k keys (32 / 8 heads, d
 // 128, bf16) take 122 us, 4.7 TB/s, where a large copy reaches 4.8.  Chosen pages of a
 // prompt's rows are bound by the L2, each row having a list of its own.
 #include "ssa_cache_attend_dev.h"
@@ -168,7 +168,7 @@ AttendShape attend_shape(const ssa_cached_attention_args *a) {
     // Chunks of two tiles or more for each wave.  Lists of pages are equally long: as
     // many workgroups as the chip holds at once (512: 32 rows of 32 pages 34.7 us, with
     // 2,048 39.2 us).  Lengths are not: smaller chunks even them out (2,048: 16 tokens
-    // over up to 32k keys 124 us, with 512 128 us, with 4,096 131 us).
+    // over 5k to 32k keys 124 us, with 512 128 us, with 4,096 131 us).
     split_tiles(tiles, s.units * c.Hkv, a->pages ? 512 : 2048, 2 * ATT_WAVES, &s.S, &s.chunk);
     // A wave a unit, where there are units enough for that: over a few keys (256 tokens
     // over 4 pages of 64: 31 us, with four waves to a unit 43 us; over 24 pages 150 us
